@@ -1357,8 +1357,9 @@ std::string plan_json(const Plan& plan) {
   }
   for (size_t p = 0; p < g.outputs.size(); ++p) {
     const Node& n = g.nodes[g.outputs[p]];
-    j << ",{\"id\":\"out" << p << "\",\"shape\":" << jshape(n.shape) << ",\"element_type\":\"" << dtype_name(n.dt)
-      << "\"}";
+    j << (first ? "" : ",") << "{\"id\":\"out" << p << "\",\"shape\":" << jshape(n.shape) << ",\"element_type\":\""
+      << dtype_name(n.dt) << "\"}";
+    first = false;
   }
   j << "],\"steps\":[";
   // One owned step per kernel; FIN kernels are steps that read their
