@@ -92,7 +92,9 @@ EXPORTED = ("fgt_last_error", "fgt_abi_version", "fgt_spec_create", "fgt_spec_de
             "fgt_comm_unique_id", "fgt_comm_create", "fgt_comm_peer_exchange", "fgt_comm_destroy",
             "fgt_spec_launch_sharded",
             "fgt_program_create", "fgt_program_run", "fgt_program_kernel_count", "fgt_program_destroy",
-            "fgt_reduce_f32_noalloc")
+            "fgt_reduce_f32_noalloc",
+            "fgt_embedding", "fgt_embedding_grad_workspace", "fgt_embedding_grad",
+            "fgt_cross_entropy_workspace", "fgt_cross_entropy", "fgt_adjust_logits")
 
 
 def check(status):

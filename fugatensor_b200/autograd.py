@@ -14,6 +14,7 @@ import builtins as _builtins
 import math
 
 from . import dtypes as _dt
+from . import operators
 from .tensor import Tensor, _prim
 
 FLOAT = ("f32", "f16", "bf16")
@@ -93,6 +94,8 @@ def _vjp(t, g, active):
     """Cotangents of t's operands given t's cotangent g (None where inactive)."""
     op, args, attrs = t._expr
     e = t.engine
+    if op in operators.NAMES:
+        return operators.vjp(t, g, active)
     if op == "add":
         return [g if a else None for a in active]
     if op == "mul":

@@ -26,7 +26,7 @@ CUDA = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
 LIB = PKG / "libfgt.so"
 
 CPP_SOURCES = ["fgt_graph.cpp", "fgt_plan.cpp", "fgt_codegen.cpp", "fgt_runtime.cpp"]
-CU_SOURCES = ["fgt_noalloc.cu"]
+CU_SOURCES = ["fgt_noalloc.cu", "fgt_embedding.cu", "fgt_loss.cu", "fgt_logits.cu"]
 HEADERS = ["fgt_internal.h", "fgt_plan.h", "fgt_driver.h", "fgt_device.cuh"]
 GENCODE = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -97,7 +97,7 @@ def build(verbose: bool = False) -> Path:
     for src in CU_SOURCES:
         src = CSRC / src
         obj = BUILD / (src.stem + ".o")
-        if _stale(obj, [src, CSRC / "fgt_device.cuh", CSRC / "fgt_driver.h", ROOT / "include" / "fgt.h"]):
+        if _stale(obj, [src, CSRC / "fgt_device.cuh", CSRC / "fgt_driver.h", CSRC / "fgt_internal.h", CSRC / "fgt_vocab.cuh", ROOT / "include" / "fgt.h"]):
             _run([str(CUDA / "bin" / "nvcc"), *GENCODE, "-lineinfo", "-O3", "-fmad=false", "-std=c++17",
                   "-Xcompiler", "-fPIC", f"-I{ROOT / 'include'}", f"-I{CSRC}", "-c", str(src), "-o", str(obj)])
         objs.append(obj)

@@ -15,6 +15,8 @@ cpp/lazy.cpp:871-1008, 946-948): the native extension runs it with the GIL
 released, and a plan of two or more kernels replays as one CUDA graph (the
 reference prepares every program with graph=True, engine.py:416-423). There
 is no CPU path and no fallback: a device without the native library raises.
+Operators (operators.py) in the graph cut it: they run as launches of their
+own between the partitions that feed them and those that read them.
 """
 from __future__ import annotations
 
@@ -22,6 +24,7 @@ import threading
 
 from . import dtypes as _dt
 from . import ir
+from .operators import NAMES as _OPERATORS
 from .tensor import Tensor
 
 _ENGINES = {}
@@ -95,8 +98,8 @@ class Engine:
         return c if tuple(shape) == () else _prim("splat", (c,), (tuple(shape),))
 
     # -- compilation -------------------------------------------------------
-    def trace(self, *tensors):
-        """Join pending tensors into one partition: (descriptor, leaves, roots)."""
+    def _roots(self, tensors):
+        """The distinct pending tensors among ``tensors``."""
         roots, seen_roots = [], set()
         for t in tensors:
             if not isinstance(t, Tensor):
@@ -106,6 +109,15 @@ class Engine:
             if t._expr is not None and id(t) not in seen_roots:
                 seen_roots.add(id(t))
                 roots.append(t)
+        return roots
+
+    def trace(self, *tensors):
+        """Join pending tensors into one partition: (descriptor, leaves, roots)."""
+        return self._trace(self._roots(tensors), {})
+
+    def _trace(self, roots, known):
+        """``trace`` of distinct pending tensors; those whose id is in ``known`` (values computed
+        earlier in the same evaluate) are leaves of the partition."""
         g = ir.Graph()
         value_of, memo, leaves = {}, {}, []
         order = []
@@ -120,12 +132,12 @@ class Engine:
                 continue
             seen.add(id(t))
             stack.append((t, True))
-            if t._expr is not None:
+            if t._expr is not None and id(t) not in known:
                 for a in reversed(t._expr[1]):
                     if id(a) not in seen:
                         stack.append((a, False))
         for t in order:
-            if t._expr is None:
+            if t._expr is None or id(t) in known:
                 v = g.parameter(t.dtype.ir, t.shape)
                 leaves.append(t)
             else:
@@ -175,29 +187,87 @@ class Engine:
         import torch
         from . import _fgt
         with self._lock:
-            desc, leaves, roots = self.trace(*tensors)
+            roots = self._roots(tensors)
+            if any(r._ops for r in roots):
+                self._evaluate_operators(roots)
+                return tensors[0] if len(tensors) == 1 else tensors
+            desc, leaves, roots = self._trace(roots, {})
             if not roots:
                 return tensors[0] if len(tensors) == 1 else tensors
             if not torch.cuda.is_available():
                 raise _fgt.CUDAError(4, "no CUDA device: fugatensor_b200 has no CPU execution path")
-            spec = self._spec(desc)
-            prog = self._program(desc.key(), spec)
             device = torch.device(self.device)
-            inputs = [t._data if t._data.device == device else t._data.to(device) for t in leaves]
             with torch.cuda.device(device):
-                outs = _fgt.run(spec, *inputs, program=prog)
+                outs = self._run_partition(desc, leaves, {}, device)
             for r, o in zip(roots, outs):
                 r._data = o
                 r._expr = None
-            plan = dict(spec.execution_plan)
-            lowering = plan.pop("cuda_lowering")
-            self.last_execution_plan = plan
-            self.last_report = {"cuda_lowering": lowering}
-            self.last_spec = spec
-            self.stats["launches"] += spec.kernel_count
-            self.stats["program_submissions"] += 1
-            self.stats["graph_replays"] += 1 if prog.graph else 0
             return tensors[0] if len(tensors) == 1 else tensors
+
+    def _run_partition(self, desc, leaves, known, device):
+        """Run one partition on the current stream and record it as the last one."""
+        from . import _fgt
+        spec = self._spec(desc)
+        prog = self._program(desc.key(), spec)
+        inputs = [known[id(t)] if id(t) in known else t._data for t in leaves]
+        outs = _fgt.run(spec, *[x if x.device == device else x.to(device) for x in inputs], program=prog)
+        plan = dict(spec.execution_plan)
+        lowering = plan.pop("cuda_lowering")
+        self.last_execution_plan = plan
+        self.last_report = {"cuda_lowering": lowering}
+        self.last_spec = spec
+        self.stats["launches"] += spec.kernel_count
+        self.stats["program_submissions"] += 1
+        self.stats["graph_replays"] += 1 if prog.graph else 0
+        return outs
+
+    def _evaluate_operators(self, roots):
+        """Evaluate roots whose graph contains operators (operators.py): launches in dependency
+        order, each after the partitions that compute what it reads, then the remaining roots as one
+        partition. Values of tensors other than the roots live for this call only: they stay pending."""
+        import torch
+        from . import _fgt, operators
+        if not torch.cuda.is_available():
+            raise _fgt.CUDAError(4, "no CUDA device: fugatensor_b200 has no CPU execution path")
+        device = torch.device(self.device)
+        known, ran = {}, []
+        self.last_execution_plan = self.last_report = None
+
+        def data(t):
+            x = known[id(t)] if t._expr is not None else t._data
+            return x if x.device == device else x.to(device)
+
+        def partition(wanted):
+            desc, leaves, outs = self._trace(wanted, known)
+            for t, o in zip(outs, self._run_partition(desc, leaves, known, device)):
+                known[id(t)] = o
+
+        with torch.cuda.device(device):
+            stream = torch.cuda.current_stream(device).cuda_stream
+            todo = operators.units(roots)
+            done = set()
+            while len(done) < len(todo):
+                ready = [i for i, (_, needs) in enumerate(todo) if i not in done and needs <= done]
+                wanted = {id(a): a for i in ready for t in todo[i][0] for a in t._expr[1]
+                          if a._expr is not None and id(a) not in known}
+                if wanted:
+                    partition(list(wanted.values()))
+                for i in ready:
+                    members = todo[i][0]
+                    for t, o in zip(members, operators.launch(members, data, stream)):
+                        known[id(t)] = o
+                        ran.append(t._expr[0])
+                    self.stats["program_submissions"] += 1
+                done.update(ready)
+            rest = [r for r in roots if id(r) not in known]
+            if rest:
+                partition(rest)
+        # of the last partition, if one ran; operators' kernels are not in it nor in stats["launches"]
+        self.last_report = {**(self.last_report or {}), "operators": ran}
+        for r in roots:
+            r._data = known[id(r)]
+            r._expr = None
+            r._ops = False
 
     def evaluate_host(self, *tensors):
         """Materialise `tensors` jointly into pinned host memory.
@@ -210,11 +280,14 @@ class Engine:
         import torch
         from . import _fgt, streaming
         with self._lock:
-            desc, leaves, roots = self.trace(*tensors)
+            roots = self._roots(tensors)
+            cut = any(r._ops for r in roots)  # operators: evaluated on the device, then downloaded
+            if not cut:
+                desc, leaves, roots = self._trace(roots, {})
             if not torch.cuda.is_available():
                 raise _fgt.CUDAError(4, "no CUDA device: fugatensor_b200 has no CPU execution path")
             device = torch.device(self.device)
-            rs = streaming.plan(self, desc, leaves, roots) if roots else None
+            rs = streaming.plan(self, desc, leaves, roots) if roots and not cut else None
             with torch.cuda.device(device):
                 if rs is None:
                     if roots:
@@ -264,6 +337,8 @@ def _hashable(attrs):
 
 
 def _build(g, op, argv, attrs):
+    if op in _OPERATORS:
+        raise TypeError(f"{op} is an operator of its own, not part of a partition: use evaluate")
     if op == "constant":
         return g.constant(attrs[0], attrs[1])
     if op == "cast":

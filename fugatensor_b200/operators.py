@@ -1,0 +1,261 @@
+"""Operators of the vocabulary: nodes of the lazy graph that run as native kernels of their own.
+
+A partition (one fused kernel list) covers the Fuga primitives; an operator
+is a pending tensor whose expression names an entry point of the C ABI
+(include/fgt.h) instead: embedding rows and their gradient, cross-entropy and
+its gradient, the rules that edit logits. ``Engine.evaluate`` cuts the graph
+at them: whatever an operator reads is evaluated first (as partitions and
+operators), and partitions take operator results as inputs. A loss and its
+gradient that are evaluated together run as one launch that reads the logits
+once.
+
+The public functions are in ``nn.functional``; this module types the nodes,
+gives their VJPs and launches them. Like partitions they run on the current
+stream, with outputs and workspaces from torch's allocator, and have no CPU
+path.
+"""
+from __future__ import annotations
+
+import numpy as np
+
+from .tensor import Tensor
+
+NAMES = frozenset(("embedding", "embedding_grad", "cross_entropy", "cross_entropy_grad", "adjust_logits"))
+REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+_DT = {"bool": 0, "i32": 1, "i64": 2, "f32": 3, "f16": 4, "bf16": 5}
+_native = None
+
+
+def node(op, args, attrs, dtype, shape):
+    """A pending tensor for operator ``op``."""
+    t = Tensor(args[0]._engine, dtype, shape, expr=(op, args, attrs))
+    t._ops = True
+    return t
+
+
+def _scalar(t, depth=4):
+    """The value of a rank-0 f32 expression of a few constants (a loss scale), or None."""
+    if t._expr is None or t._shape != () or not depth:
+        return None
+    op, args, attrs = t._expr
+    if op == "constant":
+        return float(np.float32(attrs[0]))
+    if op in ("mul", "div"):
+        a, b = (_scalar(x, depth - 1) for x in args)
+        if a is not None and b is not None:
+            with np.errstate(all="ignore"):  # as the f32 partition would compute it
+                return float(np.float32(a) * np.float32(b) if op == "mul" else np.float32(a) / np.float32(b))
+    return None
+
+
+# ------------------------------------------------------------- gradients ---
+def vjp(t, g, active):
+    """Cotangents of an operator's operands given its cotangent ``g``."""
+    op, args, attrs = t._expr
+    if op == "embedding":
+        table, indices = args
+        scale, padding = attrs
+        grad = node("embedding_grad", (indices, g), (table._shape[0], scale, padding), table._dtype, table._shape)
+        return [grad if active[0] else None, None]
+    if op == "cross_entropy":
+        logits, targets = args
+        value = _scalar(g)
+        seed, scale = ((), value) if value is not None else ((g,), 1.0)
+        return [node("cross_entropy_grad", (logits, targets) + seed, attrs + (scale,), logits._dtype, logits._shape), None]
+    from .autograd import DifferentiationError
+    raise DifferentiationError(f"{op} has no derivative rule")
+
+
+# ------------------------------------------------------------ scheduling ---
+def _pending_order(roots):
+    """The pending tensors under ``roots``, operands first."""
+    order, seen = [], set()
+    stack = [(r, False) for r in reversed(roots)]
+    while stack:
+        t, done = stack.pop()
+        if done:
+            order.append(t)
+            continue
+        if t._expr is None or id(t) in seen:
+            continue
+        seen.add(id(t))
+        stack.append((t, True))
+        for a in t._expr[1]:
+            if a._expr is not None and id(a) not in seen:
+                stack.append((a, False))
+    return order
+
+
+_NONE = frozenset()
+
+
+def units(roots):
+    """The operators under ``roots`` as launches with the launches they wait for.
+
+    Returns a list of (members, needs): ``members`` are one operator, or a
+    loss with its gradient; ``needs`` the indices of the launches whose results
+    they read, directly or through partitions. A pair is only formed when the
+    launches stay free of cycles (a seed computed from the loss itself keeps
+    the two apart)."""
+    order = _pending_order(roots)
+    found = [t for t in order if t._expr[0] in NAMES]
+    if len(found) == 1:
+        return [(found, _NONE)]
+    reads, below = {}, {}  # operators that an operator reads; that a tensor is or is computed from
+    for t in order:
+        got = _NONE
+        for a in t._expr[1]:
+            more = below.get(id(a), _NONE)
+            got = got | more if got else more
+        if t._expr[0] in NAMES:
+            reads[id(t)] = got
+            got = frozenset((id(t),))
+        below[id(t)] = got
+
+    group = {id(t): i for i, t in enumerate(found)}  # operator -> launch
+    losses = {}
+    for t in found:
+        if t._expr[0] == "cross_entropy":
+            losses[_pair_key(t)] = t
+    for t in found:
+        if t._expr[0] != "cross_entropy_grad":
+            continue
+        loss = losses.pop(_pair_key(t), None)  # one gradient per loss is paired
+        if loss is None:
+            continue
+        alone = group[id(loss)]
+        group[id(loss)] = group[id(t)]
+        if _levels(found, group, reads) is None:
+            group[id(loss)] = alone
+    ordered = _levels(found, group, reads)
+    at = {g: i for i, g in enumerate(ordered)}
+    out = [([], set()) for _ in ordered]
+    for t in found:
+        i = at[group[id(t)]]
+        out[i][0].append(t)
+        out[i][1].update(at[group[r]] for r in reads[id(t)])
+    return out
+
+
+def _pair_key(t):
+    return id(t._expr[1][0]), id(t._expr[1][1]), t._expr[2][:4]
+
+
+def _levels(found, group, reads):
+    """The launches in an order that respects ``reads``, or None if there is a cycle."""
+    needs = {}
+    for t in found:
+        needs.setdefault(group[id(t)], set()).update(group[r] for r in reads[id(t)])
+    ordered, done = [], set()
+    while len(ordered) < len(needs):
+        ready = [g for g, n in needs.items() if g not in done and n <= done]
+        if not ready:
+            return None
+        ordered += ready
+        done.update(ready)
+    return ordered
+
+
+# -------------------------------------------------------------- launches ---
+def launch(members, data, stream):
+    """Run one launch; ``data(tensor)`` gives an operand's buffer. Returns the members' results."""
+    global _native
+    if _native is None:
+        from . import _native
+    return _LAUNCH[members[-1]._expr[0]](members, data, stream)
+
+
+def _empty(t, device):
+    import torch
+    from . import _fgt
+    return torch.empty(t._shape, dtype=_fgt.torch_dtype(t._dtype.ir), device=device)
+
+
+def _buffer(t, data):
+    b = data(t)
+    if not b.is_cuda or not b.is_contiguous():
+        raise ValueError(f"operand must be a contiguous CUDA tensor, got {b.dtype}{list(b.shape)} on {b.device}")
+    return b
+
+
+def _workspace(size, device):
+    import torch
+    return torch.empty(size, dtype=torch.uint8, device=device) if size else None
+
+
+def _check(status):
+    if status:
+        from . import _fgt
+        _fgt.check(status)
+
+
+def _embedding(members, data, stream):
+    (t,) = members
+    (table, indices), (scale, padding) = t._expr[1:]
+    tb, ib = _buffer(table, data), _buffer(indices, data)
+    out = _empty(t, tb.device)
+    _check(_native.embedding(_DT[t._dtype.ir], _DT[indices._dtype.ir], table._shape[0], table._shape[1], indices.size,
+                             scale, tb.data_ptr(), ib.data_ptr(), out.data_ptr(), stream))
+    return [out]
+
+
+def _embedding_grad(members, data, stream):
+    (t,) = members
+    (indices, g), (vocab, scale, padding) = t._expr[1:]
+    ib, gb = _buffer(indices, data), _buffer(g, data)
+    out = _empty(t, gb.device)
+    desc = (_DT[t._dtype.ir], _DT[indices._dtype.ir], vocab, t._shape[1], indices.size, scale,
+            -1 if padding is None else padding)
+    size = _native.embedding_grad_workspace(*desc)
+    ws = _workspace(size, gb.device)
+    _check(_native.embedding_grad(*desc, ib.data_ptr(), gb.data_ptr(), out.data_ptr(), ws.data_ptr() if size else 0, size,
+                                  stream))
+    return [out]
+
+
+def _cross_entropy(members, data, stream):
+    loss = next((t for t in members if t._expr[0] == "cross_entropy"), None)
+    grad = next((t for t in members if t._expr[0] == "cross_entropy_grad"), None)
+    args, attrs = (loss if grad is None else grad)._expr[1:]
+    logits, targets = args[:2]
+    ignore, smoothing, z, reduction = attrs[:4]
+    xb, tb = _buffer(logits, data), _buffer(targets, data)
+    seed = _buffer(args[2], data) if len(args) == 3 else None
+    out = {id(t): _empty(t, xb.device) for t in members}
+    desc = (_DT[logits._dtype.ir], _DT[targets._dtype.ir], REDUCTIONS[reduction], smoothing, z,
+            attrs[4] if grad is not None else 1.0, targets.size, logits._shape[-1], ignore)
+    size = _native.cross_entropy_workspace(*desc)
+    ws = _workspace(size, xb.device)
+    _check(_native.cross_entropy(*desc, xb.data_ptr(), tb.data_ptr(), 0 if seed is None else seed.data_ptr(),
+                                 0 if loss is None else out[id(loss)].data_ptr(),
+                                 0 if grad is None else out[id(grad)].data_ptr(), ws.data_ptr() if size else 0, size, stream))
+    return [out[id(t)] for t in members]
+
+
+def _adjust_logits(members, data, stream):
+    (t,) = members
+    args, (names, repetition, presence, frequency) = t._expr[1:]
+    given = dict(zip(names, args))
+    kept = {k: _buffer(v, data) for k, v in given.items()}
+    out = _empty(t, kept["logits"].device)
+
+    def ptr(name):
+        return kept[name].data_ptr() if name in kept else 0
+
+    def kind(name):
+        return _DT[given[name]._dtype.ir] if name in given else 1
+
+    vocab = t._shape[-1] if t._shape else 0
+    rows = t.size // vocab if vocab else 0
+    history = given["tokens"]._shape[-1] if "tokens" in given else 0
+    biases = given["bias"]._shape[-1] if "bias" in given else 0
+    _check(_native.adjust_logits(
+        _DT[t._dtype.ir], kind("tokens"), kind("lengths" if "lengths" in given else "prompt_lengths"), kind("bias_tokens"),
+        rows, vocab, history, biases, repetition, presence, frequency, ptr("logits"), ptr("tokens"), ptr("lengths"),
+        ptr("prompt_lengths"), ptr("repetition"), ptr("presence"), ptr("frequency"), ptr("bias_tokens"), ptr("bias"),
+        ptr("allowed"), out.data_ptr(), stream))
+    return [out]
+
+
+_LAUNCH = {"embedding": _embedding, "embedding_grad": _embedding_grad, "cross_entropy": _cross_entropy,
+           "cross_entropy_grad": _cross_entropy, "adjust_logits": _adjust_logits}

@@ -16,7 +16,8 @@ from . import ir
 
 
 class Tensor:
-    __slots__ = ("_engine", "_dtype", "_shape", "_data", "_expr", "__weakref__")
+    # _ops: the pending expression may contain operators (operators.py), at which evaluate cuts the graph
+    __slots__ = ("_engine", "_dtype", "_shape", "_data", "_expr", "_ops", "__weakref__")
 
     def __init__(self, engine, dtype, shape, data=None, expr=None):
         self._engine = engine
@@ -24,6 +25,7 @@ class Tensor:
         self._shape = tuple(int(s) for s in shape)
         self._data = data
         self._expr = expr
+        self._ops = False
 
     # -- metadata ----------------------------------------------------------
     @property
@@ -396,7 +398,9 @@ def _prim(op, args, attrs=()):
         elif a._engine is not engine:
             raise ValueError("tensors belong to different engines")
     dtype, shape = _infer(op, args, attrs)
-    return Tensor(engine, _dt.BY_IR[dtype], shape, expr=(op, tuple(args), tuple(attrs)))
+    t = Tensor(engine, _dt.BY_IR[dtype], shape, expr=(op, tuple(args), tuple(attrs)))
+    t._ops = any(a._ops for a in args)
+    return t
 
 
 def _prim_on(engine, op, attrs):

@@ -1,6 +1,7 @@
 /*
  * fgt.h — C ABI of the B200-native (sm_100a) backend for FugaTensor's fused
- * elementwise / broadcast / reduction partitions.
+ * elementwise / broadcast / reduction partitions, and of the vocabulary
+ * operators (embedding, cross-entropy, logit rules) that run between them.
  *
  * A partition is a small SSA DAG of Fuga primitives (the ops that the
  * reference lowers to ASK "owned" kernels, src/fugatensor/lowering.py:88-111).
@@ -354,6 +355,107 @@ fgt_status fgt_spec_launch_sharded(const fgt_spec* spec, fgt_comm* comm, const v
  *     pending) without launching. */
 fgt_status fgt_reduce_f32_noalloc(const float* x, int64_t n, float* sum, float* max, int64_t* argmax, float* mean,
                                   void* stream);
+
+/* ---- vocabulary operators ----------------------------------------------- */
+/* The ends of a language model that touch its whole vocabulary: embedding
+ * rows in, logits out. Conventions as above: dense row-major buffers, 16-byte
+ * aligned, caller-owned; nothing is allocated; validation before any launch;
+ * launches are asynchronous on `stream` and capturable in a CUDA graph.
+ * Outputs must not overlap inputs. Index types are FGT_I32 or FGT_I64,
+ * element types FGT_F32, FGT_F16 or FGT_BF16. Sums are kept in f32 and every
+ * output value is rounded once; results do not depend on the order in which
+ * the GPU runs the work (no floating-point atomics). */
+
+typedef struct fgt_embedding_desc {
+  int32_t dtype;          /* table, out, dy and dtable                              */
+  int32_t index_dtype;
+  int64_t vocab;          /* table rows                                             */
+  int64_t dim;            /* row length                                             */
+  int64_t count;          /* indices                                                */
+  int64_t padding_index;  /* its row gets no gradient (-1: none)                    */
+  float scale;
+  int32_t reserved;
+} fgt_embedding_desc;
+
+/* out[i, :] = scale * table[indices[i], :]; indices outside [0, vocab) read 0. */
+fgt_status fgt_embedding(const fgt_embedding_desc* desc, const void* table, const void* indices, void* out,
+                         void* stream);
+
+/* dtable[v, :] = scale * (sum of dy[i, :] over indices[i] == v); rows without an
+ * index, and the padding row, are 0. Every element of dtable is written. The
+ * workspace holds the sorted indices (fgt_embedding_grad_workspace bytes). */
+fgt_status fgt_embedding_grad_workspace(const fgt_embedding_desc* desc, size_t* bytes);
+fgt_status fgt_embedding_grad(const fgt_embedding_desc* desc, const void* indices, const void* dy, void* dtable,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
+typedef enum fgt_loss_reduction { FGT_LOSS_NONE = 0, FGT_LOSS_SUM = 1, FGT_LOSS_MEAN = 2 } fgt_loss_reduction;
+
+typedef struct fgt_cross_entropy_desc {
+  int32_t dtype;          /* logits and dlogits                                     */
+  int32_t target_dtype;
+  int32_t reduction;      /* fgt_loss_reduction                                     */
+  float label_smoothing;  /* e, in [0, 1]                                           */
+  float z_loss;           /* z, >= 0: weight of lse^2                               */
+  float grad_scale;       /* multiplies the seed                                    */
+  int64_t rows;
+  int64_t vocab;
+  int64_t ignore_index;   /* rows with this target, or one outside [0, vocab),      */
+                          /* have loss and gradient 0 and are not counted           */
+} fgt_cross_entropy_desc;
+
+/* With lse = log(sum_v exp(logits[i, v])) and t = targets[i]:
+ *   loss_i = lse - (1 - e) logits[i, t] - (e / vocab) sum_v logits[i, v] + z lse^2
+ *   dlogits[i, v] = g_i (softmax_v (1 + 2 z lse) - (1 - e) [v = t] - e / vocab)
+ * loss holds f32: every row's (NONE), their sum, or the sum over the counted
+ * rows' number (MEAN; 0 when no row counts). seed is f32, the loss's
+ * cotangent: [rows] for NONE, one value otherwise, or NULL for 1; g_i is
+ * grad_scale * seed, over the number of counted rows for MEAN. loss or
+ * dlogits may be NULL (not computed); with both, the logits are read once. */
+fgt_status fgt_cross_entropy_workspace(const fgt_cross_entropy_desc* desc, size_t* bytes);
+fgt_status fgt_cross_entropy(const fgt_cross_entropy_desc* desc, const void* logits, const void* targets,
+                             const float* seed, float* loss, void* dlogits, void* workspace, size_t workspace_bytes,
+                             void* stream);
+
+typedef struct fgt_adjust_logits_desc {
+  int32_t dtype;          /* logits and out                                         */
+  int32_t token_dtype;    /* tokens                                                 */
+  int32_t length_dtype;   /* lengths and prompt_lengths                             */
+  int32_t bias_dtype;     /* bias_tokens (an index type)                            */
+  int64_t rows;
+  int64_t vocab;
+  int64_t history;        /* columns of tokens                                      */
+  int64_t biases;         /* columns of bias_tokens and bias                        */
+  float repetition;       /* used where the buffer of the same name is NULL         */
+  float presence;
+  float frequency;
+  int32_t reserved;
+} fgt_adjust_logits_desc;
+
+typedef struct fgt_adjust_logits_buffers {
+  const void* logits;         /* [rows, vocab]                                      */
+  const void* tokens;         /* [rows, history] or NULL: no history                */
+  const void* lengths;        /* [rows] or NULL: every row is `history` long        */
+  const void* prompt_lengths; /* [rows] or NULL: no row has a prompt                */
+  const float* repetition;    /* [rows] or NULL                                     */
+  const float* presence;
+  const float* frequency;
+  const void* bias_tokens;    /* [rows, biases] or NULL                             */
+  const float* bias;          /* [rows, biases] or NULL                             */
+  const uint32_t* allowed;    /* [rows, ceil(vocab / 32)] or NULL: bit v % 32 of    */
+                              /* word v / 32 set = token v may be chosen            */
+  void* out;                  /* [rows, vocab]                                      */
+} fgt_adjust_logits_buffers;
+
+/* Row b's tokens[b, 0 .. prompt_lengths[b]) are its prompt, those up to
+ * lengths[b] were generated (lengths are clamped to [0, history], prompt
+ * lengths to [0, length]); tokens outside [0, vocab) are skipped. With c(v)
+ * the count of v among the generated tokens, in this order:
+ *   v in the prompt or generated: x = x > 0 ? x / repetition : x * repetition
+ *   x = x - frequency * c(v);  c(v) > 0: x = x - presence
+ *   x = x + sum of bias[b, k] over bias_tokens[b, k] == v (in the order of k)
+ *   bit v of allowed[b] clear: x = -inf, whatever x was
+ * computed in f32 and rounded once. A row that allows nothing is all -inf. */
+fgt_status fgt_adjust_logits(const fgt_adjust_logits_desc* desc, const fgt_adjust_logits_buffers* buffers, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,382 @@
+"""Vocabulary operators (embedding, cross_entropy, adjust_logits) against 64-bit references."""
+import math
+
+import pytest
+import torch
+
+import fugatensor_b200 as ft
+import fugatensor_b200.nn.functional as F
+from tests import _vocab as R
+
+pytestmark = pytest.mark.gpu
+DTYPES = ["f32", "f16", "bf16"]
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def randn(shape, dtype, g, scale=1.0):
+    return (torch.randn(shape, device="cuda", generator=g) * scale).to(R.TORCH[dtype])
+
+
+def randint(lo, hi, shape, dtype, g):
+    return torch.randint(lo, hi, shape, device="cuda", generator=g, dtype=R.TORCH[dtype])
+
+
+# ------------------------------------------------------------- embedding ---
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("index", ["i32", "i64"])
+@pytest.mark.parametrize("shape,vocab,dim", [((1,), 1, 1), ((7,), 100, 3), ((2, 33), 1000, 8), ((3, 5, 7), 50, 511),
+                                             ((300,), 2000, 1024), ((9,), 40, 4096), ((5,), 0, 16), ((0,), 10, 16), ((4,), 10, 0)])
+def test_embedding(dtype, index, shape, vocab, dim):
+    g = gen(1)
+    table = randn((vocab, dim), dtype, g)
+    ids = randint(-2, vocab + 2, shape, index, g)
+    for scale in (1.0, -3.7):
+        out = F.embedding(R.wrap(table), R.wrap(ids), scale=scale)
+        assert out.shape == shape + (dim,) and out.dtype is R.FT[dtype] and out.is_pending
+        scale = float(torch.tensor(scale))  # the kernel's f32
+        ref = R.embedding(table, ids, scale)
+        R.check(out.torch(), ref, R.rounded(R.U32 * ref.abs(), ref, dtype))
+
+
+def test_embedding_keeps_nan_and_infinities():
+    table = torch.tensor([[math.nan, math.inf, -math.inf, 0.0], [1.0, 2.0, 3.0, 4.0]], device="cuda")
+    ids = torch.tensor([1, 0, -1], device="cuda")
+    out = F.embedding(R.wrap(table), R.wrap(ids), scale=2.0).torch()
+    assert out[0].tolist() == [2.0, 4.0, 6.0, 8.0] and out[2].tolist() == [0.0] * 4
+    assert math.isnan(out[1, 0]) and out[1, 1:].tolist() == [math.inf, -math.inf, 0.0]
+
+
+def ids_like(kind, n, vocab, g, index):
+    if kind == "one":  # every token is the same one: a single sum of n rows
+        return torch.full((n,), vocab // 2, device="cuda", dtype=R.TORCH[index])
+    if kind == "text":
+        u = torch.rand(n, device="cuda", generator=g, dtype=torch.float64)
+        return ((vocab + 1.0) ** u - 1.0).floor().clamp(0, vocab - 1).to(R.TORCH[index])
+    if kind == "mixed":  # some outside the table, runs of several lengths
+        return randint(-3, vocab + 3, (n,), index, g).div(3, rounding_mode="floor") * 3
+    return randint(0, vocab, (n,), index, g)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", ["one", "text", "mixed", "uniform"])
+@pytest.mark.parametrize("n,vocab,dim", [(1, 1, 1), (33, 5, 3), (300, 1000, 64), (2049, 333, 511), (5000, 70000, 40)])
+def test_embedding_grad(dtype, kind, n, vocab, dim):
+    g = gen(2)
+    index = "i64" if n % 2 else "i32"
+    ids = ids_like(kind, n, vocab, g, index)
+    dy = randn((n, dim), dtype, g)
+    table = R.wrap(torch.zeros(vocab, dim, device="cuda", dtype=R.TORCH[dtype]))
+    for scale, padding in ((1.0, None), (2.5, vocab // 2)):
+        y = F.embedding(table, R.wrap(ids), scale=scale, padding_idx=padding)
+        got = ft.grad(y, table, seed=R.wrap(dy))
+        assert got.shape == (vocab, dim) and got.dtype is R.FT[dtype]
+        ref, size = R.embedding_grad(ids, dy, vocab, scale, padding)
+        R.check(got.torch(), ref, R.rounded(R.U32 * size, ref, dtype))
+        again = ft.grad(F.embedding(table, R.wrap(ids), scale=scale, padding_idx=padding), table, seed=R.wrap(dy))
+        assert torch.equal(got.torch(), again.torch())  # no order of atomics in it
+
+
+@pytest.mark.parametrize("n,vocab,dim", [(40000, 300, 72), (70000, 131071, 16), (200000, 1000, 9), (131072, 300000, 4)])
+def test_embedding_grad_of_long_batches(n, vocab, dim):
+    g = gen(3)
+    ids = ids_like("text", n, vocab, g, "i32")
+    ids[::5] = 7  # a fifth of the batch is one token
+    ids[1::97] = -1
+    dy = randn((n, dim), "bf16", g)
+    table = R.wrap(torch.zeros(vocab, dim, device="cuda", dtype=torch.bfloat16))
+    got = ft.grad(F.embedding(table, R.wrap(ids)), table, seed=R.wrap(dy)).torch()
+    ref, size = R.embedding_grad(ids, dy, vocab, 1.0, None)
+    R.check(got, ref, R.rounded(R.U32 * size, ref, "bf16"))
+
+
+def test_embedding_grad_without_tokens_is_zero():
+    table = R.wrap(torch.randn(50, 24, device="cuda"))
+    for ids in (torch.empty(0, device="cuda", dtype=torch.int32), torch.full((5,), -1, device="cuda", dtype=torch.int64)):
+        got = ft.grad(F.embedding(table, R.wrap(ids)), table, seed=R.wrap(torch.ones(*ids.shape, 24, device="cuda")))
+        assert torch.equal(got.torch(), torch.zeros(50, 24, device="cuda"))
+
+
+def test_embedding_gradient_matches_differences():
+    """y is linear in the table, so a difference of any step is the derivative up to rounding."""
+    g = gen(4)
+    table, ids, dy = randn((6, 5), "f32", g), randint(0, 6, (20,), "i64", g), randn((20, 5), "f32", g)
+    T = R.wrap(table)
+    grad = ft.grad(F.embedding(T, R.wrap(ids), scale=1.5), T, seed=R.wrap(dy)).torch()
+
+    def value(t):
+        return float((F.embedding(R.wrap(t), R.wrap(ids), scale=1.5).torch().double() * dy.double()).sum())
+
+    size = float(dy.double().abs().sum()) * 1.5 * 8.0
+    for v, c in ((0, 0), (3, 4), (5, 2)):
+        up, down = table.clone(), table.clone()
+        up[v, c], down[v, c] = 4.0, -4.0
+        assert abs((value(up) - value(down)) / 8.0 - float(grad[v, c])) <= 40 * R.U32 * size
+
+
+# --------------------------------------------------------- cross-entropy ---
+def loss_case(rows, vocab, dtype, index, g, spread=3.0):
+    x = randn((rows, vocab), dtype, g, spread)
+    t = randint(0, vocab, (rows,), index, g)
+    if rows > 2:
+        t[1], t[rows // 2] = -100, vocab  # ignored, and outside
+    return x, t
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (3, 2), (5, 31), (64, 1000), (17, 1023), (9, 4097), (6, 32000), (7, 50021), (2, 300001)])
+@pytest.mark.parametrize("eps,z", [(0.0, 0.0), (0.1, 1e-2)])
+def test_cross_entropy(dtype, reduction, rows, vocab, eps, z):
+    g = gen(5)
+    x, t = loss_case(rows, vocab, dtype, "i32" if rows % 2 else "i64", g)
+    seed = None
+    if reduction == "none" or dtype == "f16":
+        seed = 0.5 + torch.rand((rows,) if reduction == "none" else (), device="cuda", generator=g)
+    loss, lbound, grad, gbound = R.cross_entropy(x, t, -100, eps, z, reduction, seed)
+    X, T = R.wrap(x), R.wrap(t)
+
+    def make():
+        out = F.cross_entropy(X, T, label_smoothing=eps, z_loss=z, reduction=reduction)
+        return out, ft.grad(out, X, seed=None if seed is None else R.wrap(seed))
+
+    l, d = make()
+    assert l.dtype is ft.fp32 and d.dtype is R.FT[dtype] and d.shape == x.shape
+    ft.evaluate(l, d)
+    assert l.engine.last_report["operators"] == ["cross_entropy", "cross_entropy_grad"]
+    R.check(l.torch(), loss, lbound + R.U32 * loss.abs(), "loss")
+    R.check(d.torch(), grad, R.rounded(gbound, grad, dtype), "gradient")
+    alone, grad_alone = make()[0], make()[1]
+    R.check(alone.torch(), loss, lbound + R.U32 * loss.abs(), "loss alone")
+    R.check(grad_alone.torch(), grad, R.rounded(gbound, grad, dtype), "gradient alone")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_cross_entropy_of_masked_logits(dtype):
+    """Columns at -inf or the type's lowest value take no part; a target there has loss inf."""
+    g = gen(6)
+    x, t = loss_case(8, 515, dtype, "i32", g)
+    low = torch.finfo(x.dtype).min
+    x[:, 100:200] = -math.inf
+    x[:, 200:300] = low
+    t[0], t[3] = 150, 50
+    x[5] = -math.inf
+    t[5] = 3          # nothing left: NaN
+    x[6] = low
+    t[6] = 9          # all at the lowest value: a uniform distribution
+    x[1, 7] = math.nan  # in an ignored row
+    x[2, 11] = math.nan  # in a counted row
+    t[2] = 5
+    loss, lbound, grad, gbound = R.cross_entropy(x, t, reduction="none")
+    X, T = R.wrap(x), R.wrap(t)
+    l = F.cross_entropy(X, T, reduction="none")
+    d = ft.grad(l, X, seed=R.wrap(torch.ones(8, device="cuda")))
+    ft.evaluate(l, d)
+    # at the lowest value lse = x + log(515) is all rounding: only its size is held
+    lbound[6] = 4 * abs(low) * R.U32
+    grad[0, 150] = grad[0, 150].nan_to_num()
+    R.check(l.torch(), loss, lbound + R.U32 * loss.abs().nan_to_num(posinf=0.0))
+    keep = torch.arange(8, device="cuda") != 6
+    R.check(d.torch()[keep], grad[keep], R.rounded(gbound[keep], grad[keep], dtype))
+    uniform = torch.full((515,), 1.0 / 515, device="cuda", dtype=torch.float64)
+    uniform[9] -= 1.0
+    R.check(d.torch()[6], uniform, R.rounded(4 * R.SUM_UNITS * uniform.abs(), uniform, dtype))
+
+
+def test_cross_entropy_when_no_row_counts():
+    x = torch.full((3, 40), math.nan, device="cuda")
+    for t in (torch.full((3,), -100, device="cuda"), torch.tensor([40, -1, 99], device="cuda")):
+        X = R.wrap(x)
+        l = F.cross_entropy(X, R.wrap(t))
+        d = ft.grad(l, X)
+        ft.evaluate(l, d)
+        assert l.item() == 0.0 and torch.equal(d.torch(), torch.zeros_like(x))
+    empty = F.cross_entropy(R.wrap(torch.zeros(0, 40, device="cuda")), R.wrap(torch.zeros(0, device="cuda", dtype=torch.int64)))
+    assert empty.item() == 0.0
+
+
+def test_cross_entropy_ignore_index_inside_the_vocabulary():
+    g = gen(7)
+    x, t = randn((50, 90), "f32", g), randint(0, 3, (50,), "i64", g)
+    loss, lbound, grad, gbound = R.cross_entropy(x, t, ignore=0)
+    X = R.wrap(x)
+    l = F.cross_entropy(X, R.wrap(t), ignore_index=0)
+    d = ft.grad(l, X)
+    ft.evaluate(l, d)
+    R.check(l.torch(), loss, lbound)
+    R.check(d.torch(), grad, R.rounded(gbound, grad, "f32"))
+
+
+def test_cross_entropy_gradient_matches_differences():
+    g = gen(8)
+    x, t = randn((4, 37), "f32", g), randint(0, 37, (4,), "i64", g)
+    X = R.wrap(x)
+    kw = dict(label_smoothing=0.2, z_loss=0.05, reduction="sum")
+    grad = ft.grad(F.cross_entropy(X, R.wrap(t), **kw), X).torch()
+    h = 2.0 ** -6
+    for r, c in ((0, 0), (1, int(t[1])), (3, 36)):
+        up, down = x.clone(), x.clone()
+        up[r, c] += h
+        down[r, c] -= h
+        a, b = (F.cross_entropy(R.wrap(v), R.wrap(t), **kw).item() for v in (up, down))
+        step = (float(up[r, c]) - float(down[r, c])) / 2
+        # f32 losses of size < 64 over 2h; third derivative of lse + z lse^2 below 1 here
+        assert abs((a - b) / (2 * step) - float(grad[r, c])) <= 64 * 2 * R.U32 / (2 * h) + h * h
+
+
+def test_loss_scale_and_seed_from_the_loss_itself():
+    """A constant seed is folded; one computed from the loss keeps loss and gradient apart."""
+    g = gen(9)
+    x, t = loss_case(12, 200, "f32", "i64", g)
+    X, T = R.wrap(x), R.wrap(t)
+    l = F.cross_entropy(X, T)
+    scaled = ft.grad(l * 8.0, X)
+    squared = ft.grad(l * l, X)
+    ft.evaluate(l, scaled, squared)
+    loss, lbound, grad, gbound = R.cross_entropy(x, t)
+    R.check(l.torch(), loss, lbound)
+    R.check(scaled.torch(), 8 * grad, R.rounded(8 * gbound, 8 * grad, "f32"))
+    R.check(squared.torch(), 2 * loss * grad, R.rounded(8 * (gbound * loss + grad.abs() * lbound), 2 * loss * grad, "f32"))
+
+
+# --------------------------------------------------------- logit rules -----
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("index", ["i32", "i64"])
+@pytest.mark.parametrize("rows,vocab,history,biases", [(1, 1, 1, 1), (3, 33, 7, 2), (2, 4096, 0, 0), (5, 4097, 100, 0), (4, 32000, 1, 50),
+                                                       (3, 50021, 3001, 300), (1, 128000, 20000, 3), (2, 300, 70000, 1000)])
+def test_adjust_logits(dtype, index, rows, vocab, history, biases):
+    g = gen(10)
+    x = randn((rows, vocab), dtype, g, 3.0)
+    tokens = ids_like("text", rows * history, vocab, g, index).reshape(rows, history)
+    tokens[:, ::11] = -1
+    tokens[:, 5::13] = vocab
+    lengths = randint(-1, history + 3, (rows,), index, g)
+    prompt = randint(-1, max(1, history), (rows,), index, g)
+    rep, pres, freq = (torch.rand(rows, device="cuda", generator=g) + o for o in (0.7, 0.0, -0.3))
+    btok = randint(-1, max(1, min(vocab, 200)) + 1, (rows, biases), index, g)
+    bias = randn((rows, biases), "f32", g, 4.0)
+    words = randint(-2 ** 31, 2 ** 31, (rows, -(-vocab // 32)), "i32", g)
+    if rows > 1:
+        words[0] = 0  # this row allows nothing
+    kw = dict(prompt_lengths=prompt, repetition=rep, presence=pres, frequency=freq, bias_tokens=btok, bias=bias, allowed=words)
+    variants = [kw, dict(kw, allowed=None), dict(allowed=words), dict(repetition=1.3, presence=0.5, frequency=0.25),
+                dict(bias_tokens=btok, bias=bias)]
+    for n, options in enumerate(variants):
+        has = n in (0, 1, 3)
+        t, le = (tokens if has else None), (lengths if n < 2 else None)
+        out = F.adjust_logits(R.wrap(x), R.wrap(t) if has else None, R.wrap(le) if le is not None else None,
+                              **{k: R.wrap(v) if isinstance(v, torch.Tensor) else v for k, v in options.items() if v is not None})
+        ref, bound = R.adjust_logits(x, t, le, **options)
+        R.check(out.torch(), ref, R.rounded(bound, ref, dtype), f"variant {n}")
+
+
+def test_adjust_logits_of_masked_and_infinite_logits():
+    x = torch.tensor([[math.nan, math.inf, -math.inf, -0.0, torch.finfo(torch.float32).min, 2.0]], device="cuda")
+    tokens = torch.tensor([[4, 1, 2, 0]], device="cuda")
+    allowed = torch.tensor([[0b111110]], device="cuda", dtype=torch.int32)
+    out = F.adjust_logits(R.wrap(x), R.wrap(tokens), repetition=2.0, frequency=1.0, allowed=R.wrap(allowed)).torch()[0]
+    assert out.tolist() == [-math.inf, math.inf, -math.inf, 0.0, -math.inf, 2.0]
+    out = F.adjust_logits(R.wrap(x), R.wrap(tokens), repetition=2.0).torch()[0]
+    assert math.isnan(out[0]) and out[1:].tolist() == [math.inf, -math.inf, 0.0, -math.inf, 2.0]
+
+
+def test_adjust_logits_of_one_vector_and_of_a_batch_of_batches():
+    g = gen(11)
+    x, tokens = randn((2, 3, 70), "f32", g), randint(0, 70, (2, 3, 9), "i32", g)
+    out = F.adjust_logits(R.wrap(x), R.wrap(tokens), repetition=1.5, presence=0.25).torch()
+    for i in range(2):
+        for j in range(3):
+            one = F.adjust_logits(R.wrap(x[i, j].clone()), R.wrap(tokens[i, j].clone()), repetition=1.5, presence=0.25)
+            assert torch.equal(one.torch(), out[i, j])
+    none = F.adjust_logits(R.wrap(x), repetition=1.5, presence=0.25).torch()
+    assert torch.equal(none, x)
+
+
+def test_biases_of_one_token_add_in_their_order():
+    """2^24 + 1 + 1 - 2^24 in f32, in order, is 0; any other association gives 2."""
+    x = torch.zeros(1, 10, device="cuda")
+    btok = torch.full((1, 4), 3, device="cuda", dtype=torch.int32)
+    bias = torch.tensor([[2.0 ** 24, 1.0, 1.0, -2.0 ** 24]], device="cuda")
+    out = F.adjust_logits(R.wrap(x), bias_tokens=R.wrap(btok), bias=R.wrap(bias)).torch()
+    assert out[0, 3] == 0.0 and float(out.abs().sum()) == 0.0
+
+
+# ---------------------------------------------------- in the lazy graph ----
+def test_operators_between_partitions():
+    """table -> scaled embedding -> layer norm -> logits by broadcast product -> loss, and the
+    gradients of both parameters, against torch's autograd in 64 bits."""
+    g = gen(12)
+    table, weight = randn((40, 16), "f32", g), randn((16, 40), "f32", g)
+    ids, t = randint(0, 40, (11,), "i64", g), randint(0, 40, (11,), "i64", g)
+    T, W = R.wrap(table), R.wrap(weight)
+    h = F.layer_norm(F.embedding(T, R.wrap(ids), scale=4.0))
+    prod = ft.broadcast_in_dim(h, (11, 16, 40), (0, 1)) * ft.broadcast_in_dim(W, (11, 16, 40), (1, 2))
+    loss = F.cross_entropy(ft.sum(prod, axis=1), R.wrap(t), label_smoothing=0.1)
+    dT, dW = ft.grad(loss, (T, W))
+    ft.evaluate(loss, dT, dW)
+    a, b = table.double().requires_grad_(), weight.double().requires_grad_()
+    hid = torch.nn.functional.layer_norm(a[ids] * 4.0, (16,))
+    ref = torch.nn.functional.cross_entropy(hid @ b, t, label_smoothing=0.1)
+    ref.backward()
+    for got, want in ((loss.torch(), ref.detach()), (dT.torch(), a.grad), (dW.torch(), b.grad)):
+        R.check(got, want, torch.full_like(want, 1e-5 * max(1.0, float(want.abs().max()))))
+
+
+def test_results_of_an_evaluate_do_not_cut_later_gradients():
+    g = gen(13)
+    table, ids = randn((9, 6), "f32", g), randint(0, 9, (5,), "i64", g)
+    T = R.wrap(table)
+    hidden = T * 2.0                               # a partition that the operator reads
+    y = F.embedding(hidden, R.wrap(ids))
+    out = ft.exp(y)
+    ft.evaluate(out)
+    assert hidden.is_pending and y.is_pending      # intermediate values are not kept
+    d = ft.grad(y, T, seed=R.wrap(torch.ones(5, 6, device="cuda"))).torch()
+    ref, _ = R.embedding_grad(ids, torch.ones(5, 6, device="cuda"), 9, 2.0, None)
+    assert torch.equal(d.double(), ref)
+
+
+def test_on_another_stream_and_in_a_cuda_graph():
+    g = gen(14)
+    x, t = loss_case(32, 3001, "bf16", "i32", g)
+    ids, dy = ids_like("text", 400, 500, g, "i32"), randn((400, 48), "bf16", g)
+    X, T = R.wrap(x), R.wrap(t)
+    E, I, G = R.wrap(torch.zeros(500, 48, device="cuda", dtype=torch.bfloat16)), R.wrap(ids), R.wrap(dy)
+
+    def run():
+        l = F.cross_entropy(X, T)
+        d = ft.grad(l, X)
+        e = ft.grad(F.embedding(E, I), E, seed=G)
+        a = F.adjust_logits(X, I_hist, repetition=1.2)
+        ft.evaluate(l, d, e, a)
+        return [v.torch() for v in (l, d, e, a)]
+
+    I_hist = R.wrap(randint(0, 3001, (32, 77), "i32", g))
+    want = [v.clone() for v in run()]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = run()
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = run()
+    for _ in range(2):
+        for h in held:
+            h.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, want))
+
+
+def test_evaluate_host_downloads_operator_results():
+    x = torch.randn(4, 50, device="cuda")
+    t = torch.tensor([1, 2, 3, 4], device="cuda")
+    l = F.cross_entropy(R.wrap(x), R.wrap(t), reduction="none")
+    ft.evaluate_host(l)
+    assert not l.torch().is_cuda
+    loss, lbound, _, _ = R.cross_entropy(x, t, reduction="none")
+    R.check(l.torch(), loss.cpu(), lbound.cpu())
