@@ -5,8 +5,12 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <algorithm>
 #include <cstdlib>
+#include <map>
+#include <mutex>
 #include <string>
+#include <tuple>
 
 #include "fgt.h"
 #include "fgt_device.cuh"
@@ -26,13 +30,63 @@ struct F32 {
 struct F16 {
   using S = fgt_u16;
   FGT_DEV float get(S v) { return fgt_f16_to_f32(v); }
+  FGT_DEV unsigned pair(float lo, float hi) {
+    unsigned u;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(u) : "f"(hi), "f"(lo));
+    return u;
+  }
   FGT_DEV S put(float f) { return fgt_f32_to_f16(f); }
 };
 struct BF16 {
   using S = fgt_u16;
   FGT_DEV float get(S v) { return fgt_bf16_to_f32(v); }
+  FGT_DEV unsigned pair(float lo, float hi) {
+    unsigned u;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u) : "f"(hi), "f"(lo));
+    return u;
+  }
   FGT_DEV S put(float f) { return fgt_f32_to_bf16(f); }
 };
+
+// 16 bytes of storage as f32 values, and back.
+template <class T> struct Vec {
+  static constexpr int kN = 16 / (int)sizeof(typename T::S);
+  static __device__ __forceinline__ void unpack(const uint4& u, float (&v)[kN]) {
+    const unsigned w[4] = {u.x, u.y, u.z, u.w};
+    if constexpr (sizeof(typename T::S) == 4) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = __uint_as_float(w[k]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        v[2 * k] = T::get((fgt_u16)w[k]);
+        v[2 * k + 1] = T::get((fgt_u16)(w[k] >> 16));
+      }
+    }
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&v)[kN]) {
+    unsigned w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (sizeof(typename T::S) == 4)
+        w[k] = __float_as_uint(v[k]);
+      else
+        w[k] = T::pair(v[2 * k], v[2 * k + 1]);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+
+// Programmatic dependent launch: a kernel waits for its predecessor on the
+// stream before it touches memory, and lets its successor be scheduled.
+FGT_DEV void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+FGT_DEV void grid_release() { asm volatile("griddepcontrol.launch_dependents;"); }
+
+FGT_DEV unsigned cluster_size() {
+  unsigned n;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
+  return n;
+}
 
 // An i32 or i64 array of indices or lengths (one branch, the same for a warp).
 struct Index {
@@ -103,6 +157,79 @@ template <class F> void for_dtype(int dt, F&& f) {
     case FGT_BF16: f(BF16{}); return;
   }
   fail(FGT_ERR_INVALID, "dtype must be f32, f16 or bf16");
+}
+
+// FGT_PDL=0: plain stream order (as for the generated kernels); so is a stream that is being captured.
+inline bool programmatic(cudaStream_t st) {
+  static const bool on = [] {
+    const char* e = std::getenv("FGT_PDL");
+    return !(e && std::atoi(e) == 0);
+  }();
+  if (!on) return false;
+  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+  cuda_check(cudaStreamIsCapturing(st, &cs), "cudaStreamIsCapturing");
+  return cs == cudaStreamCaptureStatusNone;
+}
+
+struct Launch {
+  cudaStream_t stream;
+  bool pdl;
+};
+
+// One launch; cluster > 1 groups that many CTAs. Kernels launched this way call grid_wait() first.
+template <class... P, class... A>
+void launch(const Launch& l, void (*kernel)(P...), unsigned grid, unsigned threads, size_t smem, unsigned cluster, A&&... args) {
+  cudaLaunchAttribute at[2] = {};
+  unsigned n = 0;
+  if (l.pdl) {
+    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    at[n].id = cudaLaunchAttributeClusterDimension;
+    at[n].val.clusterDim.x = cluster;
+    at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = l.stream;
+  cfg.attrs = at;
+  cfg.numAttrs = n;
+  cuda_check(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...), "launch");
+}
+
+// Once per kernel and device: allow `bytes` of dynamic shared memory.
+template <class K> void allow_smem(K kernel, size_t bytes) {
+  if (bytes > 48 * 1024) cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), "cudaFuncSetAttribute");
+}
+
+// How many clusters of the kernel run at once on the current device (asked once per kernel and device).
+template <class K> unsigned active_clusters(K kernel, unsigned threads, size_t smem, unsigned cluster) {
+  static std::mutex mu;
+  static std::map<std::tuple<const void*, int, size_t, unsigned>, unsigned> known;
+  int dev = 0;
+  cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
+  std::lock_guard<std::mutex> lock(mu);
+  unsigned& n = known[{(const void*)kernel, dev, smem, cluster}];
+  if (!n) {
+    cudaLaunchAttribute at = {};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = cluster;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(cluster);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    int c = 0;
+    cuda_check(cudaOccupancyMaxActiveClusters(&c, kernel, &cfg), "cudaOccupancyMaxActiveClusters");
+    n = c > 0 ? (unsigned)c : 1u;
+  }
+  return n;
 }
 
 inline unsigned blocks_for(int64_t work, int64_t per_block, const char* what) {
