@@ -30,6 +30,10 @@ struct F32 {
 struct F16 {
   using S = fgt_u16;
   FGT_DEV float get(S v) { return fgt_f16_to_f32(v); }
+  FGT_DEV void split(unsigned w, float& lo, float& hi) {
+    lo = fgt_f16_to_f32((fgt_u16)w);
+    hi = fgt_f16_to_f32((fgt_u16)(w >> 16));
+  }
   FGT_DEV unsigned pair(float lo, float hi) {
     unsigned u;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(u) : "f"(hi), "f"(lo));
@@ -40,6 +44,10 @@ struct F16 {
 struct BF16 {
   using S = fgt_u16;
   FGT_DEV float get(S v) { return fgt_bf16_to_f32(v); }
+  FGT_DEV void split(unsigned w, float& lo, float& hi) {
+    lo = __uint_as_float(w << 16);
+    hi = __uint_as_float(w & 0xffff0000u);
+  }
   FGT_DEV unsigned pair(float lo, float hi) {
     unsigned u;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u) : "f"(hi), "f"(lo));
@@ -58,10 +66,7 @@ template <class T> struct Vec {
       for (int k = 0; k < 4; ++k) v[k] = __uint_as_float(w[k]);
     } else {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        v[2 * k] = T::get((fgt_u16)w[k]);
-        v[2 * k + 1] = T::get((fgt_u16)(w[k] >> 16));
-      }
+      for (int k = 0; k < 4; ++k) T::split(w[k], v[2 * k], v[2 * k + 1]);
     }
   }
   static __device__ __forceinline__ uint4 pack(const float (&v)[kN]) {
@@ -110,7 +115,9 @@ template <class F> fgt_status guarded_call(const char* name, F&& f) noexcept {
 }
 
 inline void cuda_check(cudaError_t e, const char* what) {
-  if (e != cudaSuccess) fail(FGT_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
+  if (e == cudaSuccess) return;
+  cudaGetLastError();  // this call reports it: it is not left pending on the thread
+  fail(FGT_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
 }
 
 inline void check_buffer(const void* p, int64_t elements, const char* what) {
@@ -201,12 +208,13 @@ void launch(const Launch& l, void (*kernel)(P...), unsigned grid, unsigned threa
   cuda_check(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...), "launch");
 }
 
-// Once per kernel and device: allow `bytes` of dynamic shared memory.
+// Allows a kernel `bytes` of dynamic shared memory (48 KB, static included, need no leave).
 template <class K> void allow_smem(K kernel, size_t bytes) {
-  if (bytes > 48 * 1024) cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), "cudaFuncSetAttribute");
+  if (bytes > 32 * 1024) cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), "cudaFuncSetAttribute");
 }
 
-// How many clusters of the kernel run at once on the current device (asked once per kernel and device).
+// How many clusters (CTAs, for a cluster of 1) of the kernel run at once on the
+// current device; asked once per kernel, device and launch shape.
 template <class K> unsigned active_clusters(K kernel, unsigned threads, size_t smem, unsigned cluster) {
   static std::mutex mu;
   static std::map<std::tuple<const void*, int, size_t, unsigned>, unsigned> known;
@@ -215,18 +223,23 @@ template <class K> unsigned active_clusters(K kernel, unsigned threads, size_t s
   std::lock_guard<std::mutex> lock(mu);
   unsigned& n = known[{(const void*)kernel, dev, smem, cluster}];
   if (!n) {
-    cudaLaunchAttribute at = {};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = cluster;
-    at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(cluster);
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
     int c = 0;
-    cuda_check(cudaOccupancyMaxActiveClusters(&c, kernel, &cfg), "cudaOccupancyMaxActiveClusters");
+    if (cluster == 1) {
+      cuda_check(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&c, kernel, (int)threads, smem), "cudaOccupancyMaxActiveBlocksPerMultiprocessor");
+      c *= sm_count();
+    } else {
+      cudaLaunchAttribute at = {};
+      at.id = cudaLaunchAttributeClusterDimension;
+      at.val.clusterDim.x = cluster;
+      at.val.clusterDim.y = at.val.clusterDim.z = 1;
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(cluster);
+      cfg.blockDim = dim3(threads);
+      cfg.dynamicSmemBytes = smem;
+      cfg.attrs = &at;
+      cfg.numAttrs = 1;
+      cuda_check(cudaOccupancyMaxActiveClusters(&c, kernel, &cfg), "cudaOccupancyMaxActiveClusters");
+    }
     n = c > 0 ? (unsigned)c : 1u;
   }
   return n;
