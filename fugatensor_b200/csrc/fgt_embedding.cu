@@ -702,15 +702,13 @@ extern "C" fgt_status fgt_embedding_grad(const fgt_embedding_desc* d, const void
     while (d->vocab >> bits) ++bits;  // of the largest key, which is vocab itself
     const int passes = (bits + 8) / 9, digit_bits = (bits + passes - 1) / passes;
     const int64_t row_bytes = d->dim * dtype_size(d->dtype);
-    const int sms = sm_count();
 
     // the sort, beside CTAs that zero rows
     auto sort = [&](auto kernel, int pairs_per_thread, unsigned cluster, int sorting) {
       size_t smem = sorting ? sizeof(SortShared) + (size_t)kSortThreads * pairs_per_thread * sizeof(uint2) : 0;
       smem = std::max(smem, (size_t)kFillBits / 8);
-      allow_smem(kernel, smem);
       // as many clusters as run at once: a GPC's SMs do not all fit clusters of 8
-      const unsigned grid = cluster == 1 ? (unsigned)sms : std::max(2u, active_clusters(kernel, kSortThreads, smem, cluster)) * cluster;
+      const unsigned grid = std::max(2u, active_clusters(kernel, kSortThreads, smem, cluster)) * cluster;
       launch(l, kernel, grid, kSortThreads, smem, cluster, tk, p.wide ? keys : nullptr, sorting, digit_bits, passes, s, keys, pos, first,
              p.tiles * p.chunks, (char*)dtable, row_bytes);
     };

@@ -66,11 +66,18 @@ __global__ void __launch_bounds__(kCountThreads) loss_count(Index targets, Row r
 }
 
 // The number of counted rows (at least 1) for every lane of a full warp; whole
-// numbers below 2^24 are exact in f32, larger ones rounded once.
-__device__ __forceinline__ float counted_rows(const int* counted, fgt_i64 rows) {
-  const fgt_i64 blocks = (rows + kCountRows - 1) / kCountRows;
+// numbers below 2^24 are exact in f32, larger ones rounded once. Without
+// `counted` (few rows) the warp counts by itself.
+constexpr fgt_i64 kFewRows = 1024;
+__device__ __forceinline__ float counted_rows(const int* counted, const Index& targets, const Row& r) {
   fgt_i64 n = 0;
-  for (fgt_i64 i = threadIdx.x % 32; i < blocks; i += 32) n += counted[i];
+  if (counted) {
+    const fgt_i64 blocks = (r.rows + kCountRows - 1) / kCountRows;
+    for (fgt_i64 i = threadIdx.x % 32; i < blocks; i += 32) n += counted[i];
+  } else {
+#pragma unroll 8
+    for (int i = threadIdx.x % 32; i < (int)r.rows; i += 32) n += r.counts(targets[i]);
+  }
 #pragma unroll
   for (int m = 16; m; m >>= 1) n += __shfl_xor_sync(~0u, n, m);
   return (float)(n > 0 ? n : 1);
@@ -79,7 +86,7 @@ __device__ __forceinline__ float counted_rows(const int* counted, fgt_i64 rows) 
 // SUM / MEAN: row losses added in f64 in a fixed order, blocks of kCountRows
 // by one CTA each and the blocks' sums by the CTA that finishes last.
 __global__ void __launch_bounds__(kCountThreads)
-    loss_total(const float* losses, fgt_i64 rows, const int* counted, double* sums, unsigned* ticket, float* loss) {
+    loss_total(const float* losses, Index targets, Row r, const int* counted, double* sums, unsigned* ticket, float* loss) {
   __shared__ double s[kCountThreads / 32];
   __shared__ bool s_last;
   grid_wait();
@@ -99,7 +106,7 @@ __global__ void __launch_bounds__(kCountThreads)
 #pragma unroll
   for (int u = 0; u < kCountRows / kCountThreads; ++u) {
     const fgt_i64 i = blockIdx.x * (fgt_i64)kCountRows + u * kCountThreads + threadIdx.x;
-    if (i < rows) v += losses[i];
+    if (i < r.rows) v += losses[i];
   }
   v = block_sum(v);
   if (gridDim.x > 1) {
@@ -116,7 +123,7 @@ __global__ void __launch_bounds__(kCountThreads)
     v = block_sum(v);
   }
   if (threadIdx.x < 32) {
-    const float n = counted ? counted_rows(counted, rows) : 1.0f;
+    const float n = r.reduction == FGT_LOSS_MEAN ? counted_rows(counted, targets, r) : 1.0f;
     if (threadIdx.x == 0) *loss = (float)(v / n);
   }
 }
@@ -174,7 +181,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
   if (G == kCluster) fgt_cluster_sync();  // every CTA has started before another writes to it
 
   const float g_all = r.grad_scale * (seed && r.reduction != FGT_LOSS_NONE ? seed[0] : 1.0f) /
-                      (r.reduction == FGT_LOSS_MEAN ? counted_rows(counted, r.rows) : 1.0f);
+                      (r.reduction == FGT_LOSS_MEAN ? counted_rows(counted, targets, r) : 1.0f);
   // a row: `lead` single values, aligned vectors, then single values again
   auto lead_of = [&](fgt_i64 q) { return min((int)((N - (q * r.vocab) % N) % N), vocab); };
   auto end_of = [&](int lead) { return min((cta + 1) * per_cta, (vocab - lead) / N); };
@@ -481,7 +488,7 @@ extern "C" fgt_status fgt_cross_entropy(const fgt_cross_entropy_desc* d, const v
     const Row r{d->rows, d->vocab, d->ignore_index, d->label_smoothing, d->z_loss, d->grad_scale, d->reduction};
     const Index tg{targets, d->target_dtype == FGT_I64};
     const bool reduced = d->reduction != FGT_LOSS_NONE;
-    int* counted = d->reduction == FGT_LOSS_MEAN ? (int*)(ws + p.counted) : nullptr;
+    int* counted = d->reduction == FGT_LOSS_MEAN && d->rows > kFewRows ? (int*)(ws + p.counted) : nullptr;
     float* losses = loss && reduced ? (float*)(ws + p.losses) : loss;
     const unsigned blocks = (unsigned)std::max<int64_t>(1, p.blocks);
     // the count, or for SUM over several blocks only the ticket
@@ -496,7 +503,6 @@ extern "C" fgt_status fgt_cross_entropy(const fgt_cross_entropy_desc* d, const v
         const int per_cta = (int)((nvec + sh.ctas - 1) / sh.ctas);
         auto go = [&](auto kernel) {
           const size_t smem = (size_t)kStages * kBatch * sh.threads * 16;
-          allow_smem(kernel, smem);
           const int64_t groups = (int64_t)active_clusters(kernel, sh.threads, smem, sh.ctas) * (sh.group == kWarp ? kWarpGroups : 1);
           const int64_t used = std::min<int64_t>(groups, d->rows);
           const unsigned grid = (unsigned)(sh.group == kWarp ? (used + kWarpGroups - 1) / kWarpGroups : used * sh.ctas);
@@ -521,6 +527,6 @@ extern "C" fgt_status fgt_cross_entropy(const fgt_cross_entropy_desc* d, const v
           by_group(std::false_type{});
       });
     if (loss && reduced)
-      launch(l, loss_total, blocks, kCountThreads, 0, 1, losses, d->rows, counted, (double*)(ws + p.sums), (unsigned*)ws, loss);
+      launch(l, loss_total, blocks, kCountThreads, 0, 1, losses, tg, r, counted, (double*)(ws + p.sums), (unsigned*)ws, loss);
   });
 }

@@ -208,13 +208,9 @@ void launch(const Launch& l, void (*kernel)(P...), unsigned grid, unsigned threa
   cuda_check(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...), "launch");
 }
 
-// Allows a kernel `bytes` of dynamic shared memory (48 KB, static included, need no leave).
-template <class K> void allow_smem(K kernel, size_t bytes) {
-  if (bytes > 32 * 1024) cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), "cudaFuncSetAttribute");
-}
-
 // How many clusters (CTAs, for a cluster of 1) of the kernel run at once on the
-// current device; asked once per kernel, device and launch shape.
+// current device, and leave for its dynamic shared memory (48 KB, static
+// included, need none); asked once per kernel, device and launch shape.
 template <class K> unsigned active_clusters(K kernel, unsigned threads, size_t smem, unsigned cluster) {
   static std::mutex mu;
   static std::map<std::tuple<const void*, int, size_t, unsigned>, unsigned> known;
@@ -223,6 +219,7 @@ template <class K> unsigned active_clusters(K kernel, unsigned threads, size_t s
   std::lock_guard<std::mutex> lock(mu);
   unsigned& n = known[{(const void*)kernel, dev, smem, cluster}];
   if (!n) {
+    if (smem > 32 * 1024) cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "cudaFuncSetAttribute");
     int c = 0;
     if (cluster == 1) {
       cuda_check(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&c, kernel, (int)threads, smem), "cudaOccupancyMaxActiveBlocksPerMultiprocessor");

@@ -27,6 +27,13 @@ from . import ir
 from .operators import NAMES as _OPERATORS
 from .tensor import Tensor
 
+def _raw_stream(index):
+    """The current stream of CUDA device ``index`` as a raw handle."""
+    import torch
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # without building a Stream object
+    return torch.cuda.current_stream(index).cuda_stream if raw is None else raw(index)
+
+
 _ENGINES = {}
 _DEFAULT = ["cuda:0"]
 _LOCK = threading.RLock()
@@ -61,6 +68,7 @@ class Engine:
         self.last_execution_plan = None
         self.last_report = None
         self.last_spec = None
+        self._torch_device = None
 
     # -- tensors -----------------------------------------------------------
     def tensor(self, values, *, dtype=_dt.fp32, shape=None, host=False):
@@ -73,7 +81,13 @@ class Engine:
         from . import _fgt
         tdt = _fgt.torch_dtype(dtype.ir)
         if isinstance(values, torch.Tensor):
-            data = values.detach().to(tdt)
+            data = values.detach()
+            if data.dtype is not tdt:
+                data = data.to(tdt)
+            if data.is_cuda and not host and str(data.device) == self.device:  # already in place
+                if shape is not None:
+                    data = data.reshape(tuple(shape))
+                return Tensor(self, dtype, tuple(data.shape), data=data.contiguous())
         elif isinstance(values, np.ndarray) and dtype is _dt.bf16 and values.dtype == np.uint16:
             data = torch.from_numpy(values.astype(np.int16)).view(torch.bfloat16)
         elif isinstance(values, np.ndarray):
@@ -184,13 +198,14 @@ class Engine:
 
     def evaluate(self, *tensors):
         """Compile and materialise the requested tensors together."""
-        import torch
-        from . import _fgt
         with self._lock:
             roots = self._roots(tensors)
-            if any(r._ops for r in roots):
-                self._evaluate_operators(roots)
-                return tensors[0] if len(tensors) == 1 else tensors
+            for r in roots:
+                if r._ops:
+                    self._evaluate_operators(roots)
+                    return tensors[0] if len(tensors) == 1 else tensors
+            import torch
+            from . import _fgt
             desc, leaves, roots = self._trace(roots, {})
             if not roots:
                 return tensors[0] if len(tensors) == 1 else tensors
@@ -226,24 +241,37 @@ class Engine:
         order, each after the partitions that compute what it reads, then the remaining roots as one
         partition. Values of tensors other than the roots live for this call only: they stay pending."""
         import torch
-        from . import _fgt, operators
-        if not torch.cuda.is_available():
-            raise _fgt.CUDAError(4, "no CUDA device: fugatensor_b200 has no CPU execution path")
-        device = torch.device(self.device)
-        known, ran = {}, []
+        from . import operators
+        device = self._cuda_device()
+        index, known, ran = device.index, {}, []
         self.last_execution_plan = self.last_report = None
 
         def data(t):
             x = known[id(t)] if t._expr is not None else t._data
-            return x if x.device == device else x.to(device)
+            if x.get_device() != index:
+                x = x.to(device)
+            if not x.is_contiguous():
+                raise ValueError(f"operand must be a contiguous CUDA tensor, got {x.dtype}{list(x.shape)} with strides {x.stride()}")
+            return x
 
         def partition(wanted):
             desc, leaves, outs = self._trace(wanted, known)
             for t, o in zip(outs, self._run_partition(desc, leaves, known, device)):
                 known[id(t)] = o
 
-        with torch.cuda.device(device):
-            stream = torch.cuda.current_stream(device).cuda_stream
+        def run(members, stream):
+            for t, o in zip(members, operators.launch(members, data, stream)):
+                known[id(t)] = o
+                ran.append(t._expr[0])
+            self.stats["program_submissions"] += 1
+
+        def run_all():
+            stream = _raw_stream(index)
+            groups = operators.direct(roots)
+            if groups is not None:
+                for members in groups:
+                    run(members, stream)
+                return
             todo = operators.units(roots)
             done = set()
             while len(done) < len(todo):
@@ -253,21 +281,33 @@ class Engine:
                 if wanted:
                     partition(list(wanted.values()))
                 for i in ready:
-                    members = todo[i][0]
-                    for t, o in zip(members, operators.launch(members, data, stream)):
-                        known[id(t)] = o
-                        ran.append(t._expr[0])
-                    self.stats["program_submissions"] += 1
+                    run(todo[i][0], stream)
                 done.update(ready)
             rest = [r for r in roots if id(r) not in known]
             if rest:
                 partition(rest)
+
+        if torch.cuda.current_device() == index:
+            run_all()
+        else:
+            with torch.cuda.device(device):
+                run_all()
         # of the last partition, if one ran; operators' kernels are not in it nor in stats["launches"]
         self.last_report = {**(self.last_report or {}), "operators": ran}
         for r in roots:
             r._data = known[id(r)]
             r._expr = None
             r._ops = False
+
+    def _cuda_device(self):
+        """This engine's torch device; raises where there is none."""
+        import torch
+        if self._torch_device is None:
+            from . import _fgt
+            if not torch.cuda.is_available():
+                raise _fgt.CUDAError(4, "no CUDA device: fugatensor_b200 has no CPU execution path")
+            self._torch_device = torch.device(self.device)
+        return self._torch_device
 
     def evaluate_host(self, *tensors):
         """Materialise `tensors` jointly into pinned host memory.

@@ -197,41 +197,43 @@ def adjust_logits(logits, tokens=None, lengths=None, *, prompt_lengths=None, rep
     batch, vocab = logits._shape[:-1], logits._shape[-1]
     names, args = ["logits"], [logits]
 
-    def take(name, x, kinds, columns=()):
+    def take(name, x, kinds, shape):
         _tensor(x, name, kinds, logits)
-        if x._shape[:len(batch)] != batch or len(x._shape) != len(batch) + len(columns) or \
-                any(c is not None and c != n for c, n in zip(columns, x._shape[len(batch):])):
-            want = ", ".join([*map(str, batch), *("n" if c is None else str(c) for c in columns)])
-            raise ValueError(f"{name} must have shape [{want}], got {x._shape}")
-        if 0 not in x._shape:  # nothing in it: as if it had not been given
+        if x._shape != shape:
+            raise ValueError(f"{name} must have shape {shape}, got {x._shape}")
+        if 0 not in shape:  # nothing in it: as if it had not been given
             names.append(name)
             args.append(x)
 
-    if tokens is None and (lengths is not None or prompt_lengths is not None):
-        raise ValueError("lengths and prompt_lengths need tokens")
+    def columns(name, x, kinds):
+        _tensor(x, name, kinds, logits)
+        take(name, x, kinds, batch + x._shape[-1:])
+
     if tokens is not None:
-        take("tokens", tokens, _INDEX, (None,))
+        columns("tokens", tokens, _INDEX)
         for name, x in (("lengths", lengths), ("prompt_lengths", prompt_lengths)):
             if x is not None:
-                take(name, x, _INDEX)
-                if 0 in tokens._shape and names[-1] == name:
-                    names.pop()
-                    args.pop()
+                take(name, x, _INDEX, batch)
         if lengths is not None and prompt_lengths is not None and lengths._dtype is not prompt_lengths._dtype:
             raise TypeError("lengths and prompt_lengths must have the same dtype")
+        if 0 in tokens._shape:  # no history
+            names, args = ["logits"], [logits]
+    elif lengths is not None or prompt_lengths is not None:
+        raise ValueError("lengths and prompt_lengths need tokens")
     numbers = []
     for name, x in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
         if isinstance(x, _Tensor):
-            take(name, x, ("f32",))
-            x = 1.0
-        numbers.append(_number(x, name))
+            take(name, x, ("f32",), batch)
+            numbers.append(1.0)
+        else:
+            numbers.append(_number(x, name))
     if numbers[0] <= 0.0:
         raise ValueError("repetition must be positive")
     if (bias is None) != (bias_tokens is None):
         raise ValueError("bias and bias_tokens are given together")
     if bias is not None:
-        take("bias_tokens", bias_tokens, _INDEX, (None,))
-        take("bias", bias, ("f32",), (bias_tokens._shape[-1],))
+        columns("bias_tokens", bias_tokens, _INDEX)
+        take("bias", bias, ("f32",), bias_tokens._shape)
     if allowed is not None:
-        take("allowed", allowed, ("i32",), (-(-vocab // 32),))
+        take("allowed", allowed, ("i32",), batch + (-(-vocab // 32),))
     return _operators.node("adjust_logits", tuple(args), (tuple(names), *numbers), logits._dtype, logits._shape)

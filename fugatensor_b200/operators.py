@@ -21,15 +21,17 @@ import numpy as np
 from .tensor import Tensor
 
 NAMES = frozenset(("embedding", "embedding_grad", "cross_entropy", "cross_entropy_grad", "adjust_logits"))
+_DIRECT = ("embedding", "cross_entropy")  # differentiable in their first operand alone
 REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 _DT = {"bool": 0, "i32": 1, "i64": 2, "f32": 3, "f16": 4, "bf16": 5}
-_native = None
+_native = _fgt = torch = _TORCH = None  # loaded with the first launch
 
 
 def node(op, args, attrs, dtype, shape):
-    """A pending tensor for operator ``op``."""
-    t = Tensor(args[0]._engine, dtype, shape, expr=(op, args, attrs))
-    t._ops = True
+    """A pending tensor for operator ``op`` (dtype and shape are already in their final form)."""
+    t = Tensor.__new__(Tensor)
+    t._engine, t._dtype, t._shape = args[0]._engine, dtype, shape
+    t._data, t._expr, t._ops = None, (op, args, attrs), True
     return t
 
 
@@ -64,6 +66,18 @@ def vjp(t, g, active):
         return [node("cross_entropy_grad", (logits, targets) + seed, attrs + (scale,), logits._dtype, logits._shape), None]
     from .autograd import DifferentiationError
     raise DifferentiationError(f"{op} has no derivative rule")
+
+
+def vjp_direct(out, leaf, seed):
+    """``vjp`` of an operator that reads ``leaf`` and no pending tensor (there is no other path
+    between the two); None where that is not so."""
+    expr = out._expr
+    if expr is None or expr[0] not in _DIRECT or expr[1][0] is not leaf:
+        return None
+    for a in expr[1]:
+        if a._expr is not None:
+            return None
+    return vjp(out, seed, (True, False))[0]
 
 
 # ------------------------------------------------------------ scheduling ---
@@ -156,105 +170,127 @@ def _levels(found, group, reads):
     return ordered
 
 
+def direct(roots):
+    """``units`` where no root reads a pending tensor: no graph to order, or None if there is one."""
+    groups, losses = [], {}
+    for t in roots:
+        if t._expr[0] not in NAMES:
+            return None
+        for a in t._expr[1]:
+            if a._expr is not None:
+                return None
+        if t._expr[0] != "cross_entropy_grad":
+            groups.append([t])
+            if t._expr[0] == "cross_entropy":
+                losses[_pair_key(t)] = groups[-1]
+    for t in roots:
+        if t._expr[0] == "cross_entropy_grad":
+            group = losses.pop(_pair_key(t), None)
+            if group is None:
+                groups.append([t])
+            else:
+                group.append(t)
+    return groups
+
+
 # -------------------------------------------------------------- launches ---
 def launch(members, data, stream):
-    """Run one launch; ``data(tensor)`` gives an operand's buffer. Returns the members' results."""
-    global _native
+    """Run one launch on raw ``stream``; ``data(tensor)`` gives an operand's buffer. Returns the members' results."""
     if _native is None:
-        from . import _native
+        _load()
     return _LAUNCH[members[-1]._expr[0]](members, data, stream)
 
 
-def _empty(t, device):
+def _load():
+    global _native, _fgt, torch, _TORCH
     import torch
-    from . import _fgt
-    return torch.empty(t._shape, dtype=_fgt.torch_dtype(t._dtype.ir), device=device)
+    from . import _fgt, _native
+    _TORCH = {ir: _fgt.torch_dtype(ir) for ir in _DT}
 
 
-def _buffer(t, data):
-    b = data(t)
-    if not b.is_cuda or not b.is_contiguous():
-        raise ValueError(f"operand must be a contiguous CUDA tensor, got {b.dtype}{list(b.shape)} on {b.device}")
-    return b
+def _empty(t, like):
+    return like.new_empty(t._shape, dtype=_TORCH[t._dtype.ir])
 
 
-def _workspace(size, device):
-    import torch
-    return torch.empty(size, dtype=torch.uint8, device=device) if size else None
+def _workspace(size, like):
+    return like.new_empty((size,), dtype=torch.uint8) if size else None
 
 
 def _check(status):
     if status:
-        from . import _fgt
         _fgt.check(status)
 
 
 def _embedding(members, data, stream):
     (t,) = members
     (table, indices), (scale, padding) = t._expr[1:]
-    tb, ib = _buffer(table, data), _buffer(indices, data)
-    out = _empty(t, tb.device)
-    _check(_native.embedding(_DT[t._dtype.ir], _DT[indices._dtype.ir], table._shape[0], table._shape[1], indices.size,
+    tb, ib = data(table), data(indices)
+    out = _empty(t, tb)
+    _check(_native.embedding(_DT[t._dtype.ir], _DT[indices._dtype.ir], table._shape[0], table._shape[1], ib.numel(),
                              scale, tb.data_ptr(), ib.data_ptr(), out.data_ptr(), stream))
-    return [out]
+    return (out,)
 
 
 def _embedding_grad(members, data, stream):
     (t,) = members
     (indices, g), (vocab, scale, padding) = t._expr[1:]
-    ib, gb = _buffer(indices, data), _buffer(g, data)
-    out = _empty(t, gb.device)
-    desc = (_DT[t._dtype.ir], _DT[indices._dtype.ir], vocab, t._shape[1], indices.size, scale,
+    ib, gb = data(indices), data(g)
+    out = _empty(t, gb)
+    desc = (_DT[t._dtype.ir], _DT[indices._dtype.ir], vocab, t._shape[1], ib.numel(), scale,
             -1 if padding is None else padding)
     size = _native.embedding_grad_workspace(*desc)
-    ws = _workspace(size, gb.device)
+    ws = _workspace(size, gb)
     _check(_native.embedding_grad(*desc, ib.data_ptr(), gb.data_ptr(), out.data_ptr(), ws.data_ptr() if size else 0, size,
                                   stream))
-    return [out]
+    return (out,)
 
 
 def _cross_entropy(members, data, stream):
-    loss = next((t for t in members if t._expr[0] == "cross_entropy"), None)
-    grad = next((t for t in members if t._expr[0] == "cross_entropy_grad"), None)
+    loss = grad = None
+    for t in members:
+        if t._expr[0] == "cross_entropy":
+            loss = t
+        else:
+            grad = t
     args, attrs = (loss if grad is None else grad)._expr[1:]
     logits, targets = args[:2]
     ignore, smoothing, z, reduction = attrs[:4]
-    xb, tb = _buffer(logits, data), _buffer(targets, data)
-    seed = _buffer(args[2], data) if len(args) == 3 else None
-    out = {id(t): _empty(t, xb.device) for t in members}
+    xb, tb = data(logits), data(targets)
+    seed = data(args[2]) if len(args) == 3 else None
+    loss_out = None if loss is None else _empty(loss, xb)
+    grad_out = None if grad is None else torch.empty_like(xb)
     desc = (_DT[logits._dtype.ir], _DT[targets._dtype.ir], REDUCTIONS[reduction], smoothing, z,
-            attrs[4] if grad is not None else 1.0, targets.size, logits._shape[-1], ignore)
+            1.0 if grad is None else attrs[4], tb.numel(), logits._shape[-1], ignore)
     size = _native.cross_entropy_workspace(*desc)
-    ws = _workspace(size, xb.device)
+    ws = _workspace(size, xb)
     _check(_native.cross_entropy(*desc, xb.data_ptr(), tb.data_ptr(), 0 if seed is None else seed.data_ptr(),
-                                 0 if loss is None else out[id(loss)].data_ptr(),
-                                 0 if grad is None else out[id(grad)].data_ptr(), ws.data_ptr() if size else 0, size, stream))
-    return [out[id(t)] for t in members]
+                                 0 if loss is None else loss_out.data_ptr(), 0 if grad is None else grad_out.data_ptr(),
+                                 ws.data_ptr() if size else 0, size, stream))
+    return [loss_out if t is loss else grad_out for t in members]
 
 
 def _adjust_logits(members, data, stream):
     (t,) = members
     args, (names, repetition, presence, frequency) = t._expr[1:]
+    kept = {name: data(a) for name, a in zip(names, args)}  # alive until the launch
+    ptr = {name: b.data_ptr() for name, b in kept.items()}.get
     given = dict(zip(names, args))
-    kept = {k: _buffer(v, data) for k, v in given.items()}
-    out = _empty(t, kept["logits"].device)
 
-    def ptr(name):
-        return kept[name].data_ptr() if name in kept else 0
+    def last(name):  # an operand's last dimension, and its dtype
+        a = given.get(name)
+        return (0, 1) if a is None else (a._shape[-1] if a._shape else 0, _DT[a._dtype.ir])
 
-    def kind(name):
-        return _DT[given[name]._dtype.ir] if name in given else 1
-
-    vocab = t._shape[-1] if t._shape else 0
-    rows = t.size // vocab if vocab else 0
-    history = given["tokens"]._shape[-1] if "tokens" in given else 0
-    biases = given["bias"]._shape[-1] if "bias" in given else 0
+    x = kept["logits"]
+    out = torch.empty_like(x)
+    vocab = t._shape[-1]
+    (history, token), (biases, _), (_, bias_token) = last("tokens"), last("bias"), last("bias_tokens")
+    length = last("lengths" if "lengths" in given else "prompt_lengths")[1]
     _check(_native.adjust_logits(
-        _DT[t._dtype.ir], kind("tokens"), kind("lengths" if "lengths" in given else "prompt_lengths"), kind("bias_tokens"),
-        rows, vocab, history, biases, repetition, presence, frequency, ptr("logits"), ptr("tokens"), ptr("lengths"),
-        ptr("prompt_lengths"), ptr("repetition"), ptr("presence"), ptr("frequency"), ptr("bias_tokens"), ptr("bias"),
-        ptr("allowed"), out.data_ptr(), stream))
-    return [out]
+        _DT[t._dtype.ir], token, length, bias_token, x.numel() // vocab if vocab else 0, vocab, history, biases, repetition,
+        presence, frequency, ptr("logits"), ptr("tokens", 0), ptr("lengths", 0), ptr("prompt_lengths", 0),
+        ptr("repetition", 0), ptr("presence", 0), ptr("frequency", 0), ptr("bias_tokens", 0), ptr("bias", 0),
+        ptr("allowed", 0), out.data_ptr(), stream))
+    return (out,)
 
 
 _LAUNCH = {"embedding": _embedding, "embedding_grad": _embedding_grad, "cross_entropy": _cross_entropy,

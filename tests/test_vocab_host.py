@@ -91,6 +91,29 @@ def test_a_loss_and_its_gradient_are_one_launch_unless_the_seed_needs_the_loss()
     assert len(operators.units([other, grad])) == 2  # another loss
 
 
+def test_pairs_form_in_any_order_of_the_roots():
+    x, t = leaf((5, 7)), leaf(*TARGETS)
+    loss = F.cross_entropy(x, t)
+    one, two = ft.grad(loss, x), ft.grad(loss, x)
+    for roots in ([loss, one, two], [one, loss, two], [one, two, loss]):
+        for todo in (operators.direct(roots), [m for m, _ in operators.units(roots)]):
+            assert sorted(len(m) for m in todo) == [1, 2]
+            assert any(m is loss for m in next(m for m in todo if len(m) == 2))
+            assert sorted(id(m) for ms in todo for m in ms) == sorted(map(id, roots))
+    assert operators.direct([ft.exp(x)]) is None
+    assert operators.direct([F.cross_entropy(x * 2.0, t)]) is None
+
+
+def test_gradients_of_one_operator_are_found_directly_or_through_the_graph():
+    x, t = leaf((5, 7)), leaf(*TARGETS)
+    direct = ft.grad(F.cross_entropy(x, t), x)
+    (through,) = ft.grad((F.cross_entropy(x, t),), (x,))
+    assert direct._expr[0] == through._expr[0] == "cross_entropy_grad"
+    assert direct._expr[1][0] is through._expr[1][0] is x and direct._expr[2] == through._expr[2]
+    unrelated = ft.grad(F.cross_entropy(x, t), leaf((3,)))
+    assert unrelated.shape == (3,) and unrelated._expr[0] != "cross_entropy_grad"
+
+
 def test_crossed_pairs_do_not_deadlock():
     """Each gradient's seed is the other loss: pairing both would be a cycle."""
     x, t, y, u = leaf((5, 7)), leaf(*TARGETS), leaf((5, 9)), leaf(*TARGETS)
