@@ -1,13 +1,28 @@
 // fgt_logits.cu — rules that edit logits before a token is chosen: penalties
 // for tokens that occurred already, per-token biases, grammar masks.
+//
+// The work is a copy of the logits, bound by memory. What it needs beside them
+// is how often each token of the vocabulary occurred in the row's history. A
+// CTA edits a slice of a row: it counts its slice's tokens in shared memory
+// (one 32-bit counter per token, cleared first), reading the row's whole
+// history, and then streams its logits past the counters. A vector none of
+// whose tokens occurred is copied as it is. The few tokens with a bias are done
+// after the others, one thread each.
+#include <type_traits>
+
 #include "fgt_vocab.cuh"
 
 namespace fgt {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kSlice = 4096;             // tokens of a row that one CTA edits
-constexpr unsigned kPrompt = 0x80000000u;  // a counter's top bit: the token is in the prompt
+constexpr int kThreads = 512;
+constexpr int kBatch = 2;                  // vectors of logits per thread in flight, besides those at work
+constexpr int kHistoryBatch = 4;           // vectors of tokens per thread in flight
+constexpr int kLead = 8;                   // counters before a slice's first vector: a row's single values
+constexpr int kListed = kThreads;          // biases per row that a slice's list has room for
+constexpr unsigned kPrompt = 0x80000000u;  // a counter's top bits: the token is in the prompt,
+constexpr unsigned kBiased = 0x40000000u;  // has a bias,
+constexpr unsigned kTwice = 0x20000000u;   // has several
 
 struct Rules {
   fgt_i64 rows, vocab, history, biases, words;
@@ -17,50 +32,275 @@ struct Rules {
   const unsigned* allowed;
 };
 
+struct Listed {
+  int token;
+  float bias;
+};
+
+// For a token that occurred or has a bias. x / repetition is x times the rounded
+// reciprocal (within 1.5 units of f32), and the count's share is one FMA.
+struct Penalty {
+  float repetition, inverse, presence, frequency;
+  __device__ __forceinline__ Penalty(float r, float p, float f)
+      : repetition(r), inverse(1.0f / r), presence(p), frequency(f) {}
+  __device__ __forceinline__ float operator()(float x, unsigned count) const {
+    const unsigned made = count & ~(kPrompt | kBiased | kTwice);
+    const float less = __fmul_rn(x, x > 0.0f ? inverse : repetition);
+    x = count & ~(kBiased | kTwice) ? less : x;
+    const float lower = __fsub_rn(__fmaf_rn(-frequency, (float)made, x), presence);
+    return made ? lower : x;
+  }
+};
+
 template <class T>
-__global__ void __launch_bounds__(kThreads)
-    adjust_slices(const typename T::S* __restrict__ logits, Rules r, fgt_i64 slices, typename T::S* __restrict__ out) {
-  __shared__ unsigned count[kSlice];
-  __shared__ float bias[kSlice];
-  const fgt_i64 row = blockIdx.x / slices, v0 = blockIdx.x % slices * kSlice;
-  for (int i = threadIdx.x; i < kSlice; i += kThreads) {
-    count[i] = 0;
-    bias[i] = 0.0f;
+__global__ void __launch_bounds__(kThreads, 3)
+    adjust_slices(const typename T::S* __restrict__ logits, Rules r, int slices, int slice_vecs, typename T::S* __restrict__ out) {
+  using E = typename T::S;
+  constexpr int N = Vec<T>::kN;
+  extern __shared__ __align__(16) unsigned count[];  // [kLead + slice_vecs * N + N]
+  grid_wait();
+  grid_release();
+  const fgt_i64 row = blockIdx.x / slices;
+  const int slice = (int)(blockIdx.x % slices), vocab = (int)r.vocab;
+  // the row: `lead` single values (the first slice's), aligned vectors, single values (the last slice's)
+  const fgt_i64 e0 = row * r.vocab;
+  const int lead = min((int)((N - e0 % N) % N), vocab), nvec = (vocab - lead) / N;
+  const int first = min(slice * slice_vecs, nvec), end = slice + 1 == slices ? nvec : min(first + slice_vecs, nvec);
+  const int base = lead + first * N;  // the token of the slice's first vector: its counter is kLead
+  const int low = slice == 0 ? 0 : base, high = slice + 1 == slices ? vocab : lead + end * N;
+  const E* const x = logits + e0;
+  E* const y = out + e0;
+  const uint4* const in = reinterpret_cast<const uint4*>(x + lead);
+
+  const unsigned* const allowed = r.allowed ? r.allowed + row * r.words : nullptr;
+  uint4 u[kBatch];
+  unsigned bits[kBatch];  // of vector u: bit e set = its value e may be chosen
+  auto fetch = [&](int i0) {
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int i = i0 + b * kThreads;
+      if (i >= end) continue;
+      u[b] = __ldcs(in + i);
+      if (!allowed) continue;
+      const int t = lead + i * N;
+      bits[b] = __funnelshift_r(allowed[t >> 5], (t & 31) + N > 32 ? allowed[(t >> 5) + 1] : 0u, t & 31);
+    }
+  };
+  fetch(first + threadIdx.x);  // on its way while the history is counted
+
+  // The row's history: `before` single tokens, then 16-byte vectors of `per` tokens, then single tokens.
+  const int per = r.tokens.wide ? 2 : 4, size = 16 / per;
+  const char* const history = static_cast<const char*>(r.tokens.p) + row * r.history * size;
+  const int before = min((int)((16 - ((uintptr_t)history & 15)) & 15) / size, (int)r.history);
+  uint4 h[kHistoryBatch];
+  auto recall = [&](int i0, int vectors) {
+#pragma unroll
+    for (int b = 0; b < kHistoryBatch; ++b)
+      if (i0 + b * kThreads < vectors) h[b] = __ldcs(reinterpret_cast<const uint4*>(history + before * size) + i0 + b * kThreads);
+  };
+  if (r.tokens.p) recall(threadIdx.x, ((int)r.history - before) / per);  // before the lengths are known
+
+  // The slice's biases in their order: each warp appends its own after those of the warps before.
+  const int counters = (kLead + slice_vecs * N + N + 3) / 4 * 4;
+  Listed* const list = reinterpret_cast<Listed*>(count + counters);
+  __shared__ int s_listed[kThreads / 32];
+  const int biases = r.bias ? (int)r.biases : 0, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const bool listed = biases > 0 && biases <= kListed;
+  int bias_token = -1;
+  float bias_value = 0.0f;
+  if (listed) {
+    if ((int)threadIdx.x < biases) {
+      const fgt_i64 v = r.bias_tokens[row * r.biases + threadIdx.x];
+      bias_value = r.bias[row * r.biases + threadIdx.x];
+      if (v >= low && v < high) bias_token = (int)v;
+    }
+    const int n = __popc(__ballot_sync(~0u, bias_token >= 0));
+    if (lane == 0) s_listed[warp] = n;
   }
-  __syncthreads();
+
+  Penalty penalty(1.0f, 0.0f, 0.0f);
+  int n = 0, prompt = 0;
   if (r.tokens.p) {
-    fgt_i64 n = r.lengths.p ? r.lengths[row] : r.history;
-    n = n < 0 ? 0 : n > r.history ? r.history : n;
-    const fgt_i64 np = r.prompt_lengths.p ? r.prompt_lengths[row] : 0;
-    for (fgt_i64 i = threadIdx.x; i < n; i += kThreads) {
-      const fgt_i64 t = r.tokens[row * r.history + i];
-      if (t < v0 || t >= v0 + kSlice || t >= r.vocab) continue;
-      if (i < np)
-        atomicOr(&count[t - v0], kPrompt);
-      else
-        atomicAdd(&count[t - v0], 1u);
-    }
+    penalty = Penalty(r.repetition ? r.repetition[row] : r.repetition0, r.presence ? r.presence[row] : r.presence0,
+                      r.frequency ? r.frequency[row] : r.frequency0);
+    fgt_i64 len = r.lengths.p ? r.lengths[row] : r.history;
+    n = (int)(len < 0 ? 0 : len > r.history ? r.history : len);
+    len = r.prompt_lengths.p ? r.prompt_lengths[row] : 0;
+    prompt = (int)(len < 0 ? 0 : len > n ? n : len);
   }
-  if (threadIdx.x == 0 && r.bias)
-    for (fgt_i64 k = 0; k < r.biases; ++k) {  // in the order of k
-      const fgt_i64 t = r.bias_tokens[row * r.biases + k];
-      if (t >= v0 && t < v0 + kSlice && t < r.vocab) bias[t - v0] = __fadd_rn(bias[t - v0], r.bias[row * r.biases + k]);
-    }
+  const bool counting = r.tokens.p || listed;
+  if (counting) {
+    uint4* const clear = reinterpret_cast<uint4*>(count);
+    for (int i = threadIdx.x; i < (kLead + (end - first) * N + N) / 4; i += kThreads) clear[i] = make_uint4(0, 0, 0, 0);
+  }
   __syncthreads();
-  const float rep = r.repetition ? r.repetition[row] : r.repetition0;
-  const float pres = r.presence ? r.presence[row] : r.presence0;
-  const float freq = r.frequency ? r.frequency[row] : r.frequency0;
-  for (int i = threadIdx.x; i < kSlice; i += kThreads) {
-    const fgt_i64 v = v0 + i;
-    if (v >= r.vocab) return;
-    float x = T::get(logits[row * r.vocab + v]);
-    const unsigned c = count[i], made = c & ~kPrompt;
-    if (c) x = x > 0.0f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
-    if (made) x = __fsub_rn(__fsub_rn(x, __fmul_rn(freq, (float)made)), pres);
-    x = __fadd_rn(x, bias[i]);
-    if (r.allowed && !(r.allowed[row * r.words + (v >> 5)] >> (v & 31) & 1)) x = __int_as_float(0xff800000);
-    out[row * r.vocab + v] = T::put(x);
+  int all_listed = 0;
+  if (listed) {
+    const unsigned in_slice = __ballot_sync(~0u, bias_token >= 0);
+    int at = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+      at += w < warp ? s_listed[w] : 0;
+      all_listed += s_listed[w];
+    }
+    if (bias_token >= 0) {
+      list[at + __popc(in_slice & ((1u << lane) - 1))] = Listed{bias_token, bias_value};
+      unsigned* c = count + (bias_token - base + kLead);
+      if (atomicOr(c, kBiased) & kBiased) atomicOr(c, kTwice);
+    }
   }
+  if (n > 0) {
+    const unsigned span = (unsigned)(high - low);
+    unsigned* const counter = count + (low - base + kLead);
+    auto prompted = [&](int t) {
+      if ((unsigned)(t - low) < span) atomicOr(counter + (t - low), kPrompt);
+    };
+    auto generated = [&](int t) {
+      if ((unsigned)(t - low) < span) atomicAdd(counter + (t - low), 1u);
+    };
+    auto visit = [&](int t, int i) { i < prompt ? prompted(t) : generated(t); };
+    auto narrow = [](fgt_i64 t) { return t >> 31 ? -1 : (int)t; };  // -1: none that a vocabulary has
+    auto single = [&](int i) {
+      visit(r.tokens.wide ? narrow(reinterpret_cast<const fgt_i64*>(history)[i]) : reinterpret_cast<const int*>(history)[i], i);
+    };
+    const int vectors = n > before ? (n - before) / per : 0, after = before + vectors * per;
+    if (threadIdx.x < min(before, n)) single(threadIdx.x);
+    if (after + threadIdx.x < n) single(after + threadIdx.x);  // fewer than `per`
+    for (int i0 = threadIdx.x; i0 < vectors; i0 += kHistoryBatch * kThreads) {
+      if (i0 != threadIdx.x) recall(i0, vectors);
+#pragma unroll
+      for (int b = 0; b < kHistoryBatch; ++b) {
+        if (i0 + b * kThreads >= vectors) break;
+        const int i = before + (i0 + b * kThreads) * per;
+        if (r.tokens.wide) {
+          visit(narrow((fgt_i64)h[b].x | (fgt_i64)(int)h[b].y << 32), i);
+          visit(narrow((fgt_i64)h[b].z | (fgt_i64)(int)h[b].w << 32), i + 1);
+        } else if (i >= prompt) {
+          generated((int)h[b].x);
+          generated((int)h[b].y);
+          generated((int)h[b].z);
+          generated((int)h[b].w);
+        } else {
+          visit((int)h[b].x, i);
+          visit((int)h[b].y, i + 1);
+          visit((int)h[b].z, i + 2);
+          visit((int)h[b].w, i + 3);
+        }
+      }
+    }
+  }
+  __syncthreads();
+
+  // one value by itself: the row's single values, and tokens with a bias
+  auto edited = [&](int v, bool has_bias, float bias) {
+    if (allowed && !(allowed[v >> 5] >> (v & 31) & 1)) return T::put(__int_as_float(0xff800000));
+    const float f = penalty(T::get(x[v]), counting ? count[v - base + kLead] : 0);
+    return T::put(has_bias ? __fadd_rn(f, bias) : f);
+  };
+  // A token with a bias is stored after the others, which do without biases.
+  // Where a token has several entries, each of their threads adds all of them in
+  // their order: they store the same value.
+  E biased_value = 0;
+  if (bias_token >= 0) {
+    float sum = bias_value;
+    if (count[bias_token - base + kLead] & kTwice) {
+      sum = 0.0f;
+      for (int j = 0; j < all_listed; ++j)
+        if (list[j].token == bias_token) sum = __fadd_rn(sum, list[j].bias);
+    }
+    biased_value = edited(bias_token, true, sum);
+  }
+
+  constexpr unsigned kMinusInf = sizeof(E) == 4 ? 0xff800000u : std::is_same<T, F16>::value ? 0xfc00u : 0xff80u;
+  for (int i0 = first + threadIdx.x; i0 < end; i0 += kBatch * kThreads) {
+    uint4 now[kBatch];
+    unsigned may[kBatch];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      now[b] = u[b];
+      may[b] = bits[b];
+    }
+    fetch(i0 + kBatch * kThreads);
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int i = i0 + b * kThreads;
+      if (i >= end) break;
+      if (r.tokens.p) {
+        const uint4* c = reinterpret_cast<const uint4*>(count + kLead) + (i - first) * (N / 4);
+        uint4 n[N / 4];
+        unsigned some = 0;
+#pragma unroll
+        for (int k = 0; k < N / 4; ++k) {
+          n[k] = c[k];
+          some |= n[k].x | n[k].y | n[k].z | n[k].w;
+        }
+        if (some) {
+          float v[N];
+          Vec<T>::unpack(now[b], v);
+#pragma unroll
+          for (int k = 0; k < N / 4; ++k) {
+            // (a branch that no lane takes is worth a vote)
+            const unsigned lanes = __activemask();
+            if (__any_sync(lanes, n[k].x)) v[4 * k] = penalty(v[4 * k], n[k].x);
+            if (__any_sync(lanes, n[k].y)) v[4 * k + 1] = penalty(v[4 * k + 1], n[k].y);
+            if (__any_sync(lanes, n[k].z)) v[4 * k + 2] = penalty(v[4 * k + 2], n[k].z);
+            if (__any_sync(lanes, n[k].w)) v[4 * k + 3] = penalty(v[4 * k + 3], n[k].w);
+          }
+          now[b] = Vec<T>::pack(v);
+        }
+      }
+      if (allowed) {
+        unsigned w[4] = {now[b].x, now[b].y, now[b].z, now[b].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (sizeof(E) == 4) {
+            w[k] = may[b] >> k & 1 ? w[k] : kMinusInf;
+          } else {
+            const unsigned keep = (may[b] >> (2 * k) & 1 ? 0xffffu : 0) | (may[b] >> (2 * k + 1) & 1 ? 0xffff0000u : 0);
+            w[k] = (w[k] & keep) | (kMinusInf * 0x10001u & ~keep);
+          }
+        }
+        now[b] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      __stcs(reinterpret_cast<uint4*>(y + lead) + i, now[b]);
+    }
+  }
+
+  if (slice == 0 && threadIdx.x < lead) y[threadIdx.x] = edited(threadIdx.x, false, 0.0f);
+  const int rest = lead + nvec * N + threadIdx.x;
+  if (slice + 1 == slices && rest < vocab) y[rest] = edited(rest, false, 0.0f);
+  if (!biases) return;
+  __syncthreads();  // the values without their biases are written
+  if (listed) {
+    if (bias_token >= 0) y[bias_token] = biased_value;
+    return;
+  }
+  // more biases than the list has room for: the same from global memory
+  for (int k = threadIdx.x; k < biases; k += kThreads) {
+    const fgt_i64 v = r.bias_tokens[row * r.biases + k];
+    if (v < low || v >= high) continue;
+    float sum = 0.0f;
+    bool mine = true;
+#pragma unroll 4
+    for (int j = 0; j < biases; ++j) {
+      if (r.bias_tokens[row * r.biases + j] != v) continue;
+      mine = mine && j >= k;
+      sum = __fadd_rn(sum, r.bias[row * r.biases + j]);
+    }
+    if (mine) y[v] = edited((int)v, true, sum);
+  }
+}
+
+// Slices of a row: at most kSliceTokens tokens (three CTAs of 512 threads fit an
+// SM with their counters), and more of them where the rows are too few to give
+// every SM three CTAs, down to one vector per thread. Every slice reads the
+// row's whole history, so no more than that: 384 rows of 50021 f32 with 24576
+// tokens of history each took 61 us with 4 slices, 87 with 8.
+constexpr int64_t kSliceTokens = 16384;
+
+int slices_for(int64_t rows, int64_t vocab, int64_t per_vec) {
+  const int64_t most = std::max<int64_t>(1, vocab / (per_vec * kThreads)), least = (vocab + kSliceTokens - 1) / kSliceTokens;
+  return (int)std::max(least, std::min(most, (3 * 148 + rows - 1) / rows));
 }
 
 }  // namespace
@@ -73,13 +313,15 @@ extern "C" fgt_status fgt_adjust_logits(const fgt_adjust_logits_desc* d, const f
     require(d != nullptr && b != nullptr, "desc or buffers is NULL");
     require(is_float(d->dtype), "dtype must be f32, f16 or bf16");
     size_product(d->rows, d->vocab, "rows x vocab");
+    require(d->vocab <= 1 << 30, "vocab must be at most 2^30");
+    require(d->biases < (INT64_C(1) << 30), "a row has fewer than 2^30 biases");
     const fgt_i64 words = (d->vocab + 31) / 32;
     check_buffer(b->logits, d->rows * d->vocab, "logits");
     check_buffer(b->out, d->rows * d->vocab, "out");
     if (b->tokens) {
       check_index_dtype(d->token_dtype, "tokens");
       check_buffer(b->tokens, size_product(d->rows, d->history, "tokens"), "tokens");
-      require(d->history < kPrompt, "a history has at most 2^31 - 1 tokens");
+      require(d->history < (int64_t)kTwice, "a history has fewer than 2^29 tokens");
       if (b->lengths || b->prompt_lengths) check_index_dtype(d->length_dtype, "lengths");
       if (b->lengths) check_buffer(b->lengths, d->rows, "lengths");
       if (b->prompt_lengths) check_buffer(b->prompt_lengths, d->rows, "prompt_lengths");
@@ -104,13 +346,19 @@ extern "C" fgt_status fgt_adjust_logits(const fgt_adjust_logits_desc* d, const f
                   Index{b->prompt_lengths, d->length_dtype == FGT_I64}, Index{b->bias_tokens, d->bias_dtype == FGT_I64},
                   b->repetition, b->presence, b->frequency, b->bias, d->repetition, d->presence, d->frequency,
                   b->allowed};
-    const fgt_i64 slices = (d->vocab + kSlice - 1) / kSlice;
-    const unsigned grid = blocks_for(size_product(d->rows, slices, "rows x vocab"), 1, "rows x vocab");
     for_dtype(d->dtype, [&](auto t) {
       using T = decltype(t);
-      using S = typename T::S;
-      adjust_slices<T><<<grid, kThreads, 0, (cudaStream_t)stream>>>((const S*)b->logits, r, slices, (S*)b->out);
+      using E = typename T::S;
+      constexpr int N = Vec<T>::kN;
+      const int slices = slices_for(d->rows, d->vocab, N);
+      const int64_t nvec = d->vocab / N, slice_vecs = (nvec + slices - 1) / slices;
+      const bool listed = b->bias && d->biases <= kListed;
+      const size_t smem = (b->tokens || listed ? (size_t)(kLead + slice_vecs * N + N + 3) / 4 * 16 : 0) +
+                          (listed ? (size_t)d->biases * sizeof(Listed) : 0);
+      active_clusters(adjust_slices<T>, kThreads, smem, 1);  // leave for the shared memory
+      launch(Launch{(cudaStream_t)stream, programmatic((cudaStream_t)stream)}, adjust_slices<T>,
+             blocks_for(size_product(d->rows, slices, "rows x vocab"), 1, "rows x vocab"), kThreads, smem, 1, (const E*)b->logits,
+             r, slices, (int)slice_vecs, (E*)b->out);
     });
-    cuda_check(cudaGetLastError(), "launch");
   });
 }

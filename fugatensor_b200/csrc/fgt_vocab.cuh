@@ -214,12 +214,17 @@ void launch(const Launch& l, void (*kernel)(P...), unsigned grid, unsigned threa
 template <class K> unsigned active_clusters(K kernel, unsigned threads, size_t smem, unsigned cluster) {
   static std::mutex mu;
   static std::map<std::tuple<const void*, int, size_t, unsigned>, unsigned> known;
+  static std::map<std::pair<const void*, int>, size_t> allowed;  // one setting per kernel: it only grows
   int dev = 0;
   cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
   std::lock_guard<std::mutex> lock(mu);
   unsigned& n = known[{(const void*)kernel, dev, smem, cluster}];
   if (!n) {
-    if (smem > 32 * 1024) cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "cudaFuncSetAttribute");
+    size_t& most = allowed[{(const void*)kernel, dev}];
+    if (smem > 32 * 1024 && smem > most) {
+      cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "cudaFuncSetAttribute");
+      most = smem;
+    }
     int c = 0;
     if (cluster == 1) {
       cuda_check(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&c, kernel, (int)threads, smem), "cudaOccupancyMaxActiveBlocksPerMultiprocessor");
@@ -237,7 +242,8 @@ template <class K> unsigned active_clusters(K kernel, unsigned threads, size_t s
       cfg.numAttrs = 1;
       cuda_check(cudaOccupancyMaxActiveClusters(&c, kernel, &cfg), "cudaOccupancyMaxActiveClusters");
     }
-    n = c > 0 ? (unsigned)c : 1u;
+    require(c > 0, "a kernel does not fit the device", FGT_ERR_CUDA);
+    n = (unsigned)c;
   }
   return n;
 }

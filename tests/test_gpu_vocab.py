@@ -245,7 +245,8 @@ def test_loss_scale_and_seed_from_the_loss_itself():
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("index", ["i32", "i64"])
 @pytest.mark.parametrize("rows,vocab,history,biases", [(1, 1, 1, 1), (3, 33, 7, 2), (2, 4096, 0, 0), (5, 4097, 100, 0), (4, 32000, 1, 50),
-                                                       (3, 50021, 3001, 300), (1, 128000, 20000, 3), (2, 300, 70000, 1000)])
+                                                       (3, 50021, 3001, 300), (1, 128000, 20000, 3), (2, 300, 70000, 1000),
+                                                       (3, 70001, 33, 2500)])
 def test_adjust_logits(dtype, index, rows, vocab, history, biases):
     g = gen(10)
     x = randn((rows, vocab), dtype, g, 3.0)
