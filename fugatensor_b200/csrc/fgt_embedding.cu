@@ -11,6 +11,8 @@
 // sorted (stable, hence in the order of i), long runs of one token are cut into
 // pieces that different warps add in f32, and the last warp to finish adds the
 // pieces in their order; rows without a token are zeroed while the sort runs.
+#include <type_traits>
+
 #include "fgt_vocab.cuh"
 
 namespace fgt {
@@ -88,11 +90,15 @@ __global__ void __launch_bounds__(kLookupThreads)
 // the token, or V for tokens that have no gradient (outside the table, the
 // padding row): those end up last. Digits have at most 9 bits, so a vocabulary
 // below 2^18 takes two passes. A CTA holds kSortThreads * E pairs in shared
-// memory; each warp ranks its pairs 32 at a time with match.any, and the
-// warps' counts are summed per digit.
+// memory; each warp ranks its pairs 32 at a time (the lanes with the same
+// digit are found by one ballot per bit: match.any walks the distinct values
+// and took 2 us for a round of 32 warps), and the warps' counts are summed per
+// digit. A pass puts the CTA's pairs in order before it sends them on, so that
+// what goes to another CTA goes in runs (sent singly, a pass over 8 pairs per
+// thread spent 10,000 cycles on it).
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
-constexpr int kDigits = 512;
-constexpr int kSortCtas = 8;  // the largest portable cluster
+constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits;
+constexpr int kSortCtas = 8, kMostSortCtas = 16;  // the largest portable cluster, the largest
 
 struct Tokens {
   Index ids;
@@ -107,21 +113,22 @@ struct Tokens {
 struct SortShared {
   unsigned short hist[kSortWarps][kDigits];  // per warp: a digit's count, then its start within the CTA's
   unsigned total[kDigits];                   // per digit: the CTA's count
-  unsigned base[kDigits];                    // per digit: where the CTA's first pair goes
-  unsigned warp_sum[kDigits / 32];
+  unsigned start[kDigits];                   // per digit: its first place in the CTA
+  unsigned delta[kDigits];                   // per digit: from a place in the CTA to one among all pairs
+  unsigned warp_sum[2][kDigits / 32];
 };
 
 // Stable rank of each of a warp's E x 32 digits within the warp; hist[warp]
 // ends as the warp's counts.
-template <int E>
-__device__ __forceinline__ void rank_digits(SortShared& s, int bits, const unsigned (&digit)[E], unsigned (&rank)[E]) {
+template <int E> __device__ __forceinline__ void rank_digits(SortShared& s, const unsigned (&digit)[E], unsigned (&rank)[E]) {
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   for (int d = lane; d < kDigits; d += 32) s.hist[warp][d] = 0;
   __syncwarp();
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     unsigned same = ~0u;
-    for (int b = 0; b < bits; ++b) {
+#pragma unroll
+    for (int b = 0; b < kDigitBits; ++b) {
       const unsigned set = __ballot_sync(~0u, digit[e] >> b & 1);
       same &= digit[e] >> b & 1 ? set : ~set;
     }
@@ -151,22 +158,45 @@ __device__ __forceinline__ void scan_warps(SortShared& s) {
   }
 }
 
-// base[d] = (pairs with a smaller digit anywhere) + (pairs with digit d in the
-// CTAs before); thread d < kDigits brings both of its counts.
-__device__ __forceinline__ void scan_digits(SortShared& s, unsigned all, unsigned before) {
-  unsigned run = all;
+// start[d] = the CTA's pairs with a smaller digit; delta[d] = (pairs with a
+// smaller digit anywhere) + (pairs with digit d in the CTAs before) - start[d].
+// Thread d < kDigits brings its digit's counts: the CTA's, all, the CTAs' before.
+__device__ __forceinline__ void scan_digits(SortShared& s, unsigned own, unsigned all, unsigned before) {
+  unsigned run_own = own, run_all = all;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
 #pragma unroll
   for (int m = 1; m < 32; m <<= 1) {
-    const unsigned o = __shfl_up_sync(~0u, run, m);
-    if (lane >= m) run += o;
+    const unsigned o = __shfl_up_sync(~0u, run_own, m), a = __shfl_up_sync(~0u, run_all, m);
+    if (lane >= m) {
+      run_own += o;
+      run_all += a;
+    }
   }
-  if (threadIdx.x < kDigits && lane == 31) s.warp_sum[warp] = run;
+  if (threadIdx.x < kDigits && lane == 31) {
+    s.warp_sum[0][warp] = run_own;
+    s.warp_sum[1][warp] = run_all;
+  }
   __syncthreads();
   if (threadIdx.x < kDigits) {
-    unsigned at = run - all + before;
-    for (int w = 0; w < warp; ++w) at += s.warp_sum[w];
-    s.base[threadIdx.x] = at;
+    unsigned place = run_own - own, to = run_all - all + before;
+    for (int w = 0; w < warp; ++w) {
+      place += s.warp_sum[0][w];
+      to += s.warp_sum[1][w];
+    }
+    s.start[threadIdx.x] = place;
+    s.delta[threadIdx.x] = to - place;
+  }
+  __syncthreads();
+}
+
+// The CTA's pairs in the order of their digits, into `staged`.
+template <int E>
+__device__ __forceinline__ void stage_pairs(SortShared& s, const uint2 (&pair)[E], int shift, unsigned mask, const unsigned (&rank)[E], uint2* staged) {
+  const int warp = threadIdx.x / 32;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const unsigned d = pair[e].x >> shift & mask;
+    staged[s.start[d] + s.hist[warp][d] + rank[e]] = pair[e];
   }
   __syncthreads();
 }
@@ -186,28 +216,42 @@ struct Sums {
   const unsigned* first;       // per tile: where the run of its first pair starts
   unsigned long long* done;    // per tile that a long run starts in, and chunk: pieces finished (low half), pieces in all (high half, once known)
   float* partial;              // [2 * tiles, dim]
+  fgt_u16* present;            // per block of kBlock rows: bit k set = its row k has a token
   unsigned count, tiles, vocab;
 };
 
-// Rows without a token are zero. Blocks of 16 rows are dealt out to the
-// filling CTAs in turn, since the frequent tokens of a vocabulary lie
-// together. A CTA marks the rows of its blocks that occur: by reading all
-// tokens (through L2), so it waits for nothing, or where they are sorted
-// already by searching them.
-constexpr int kFillBits = 1 << 18;  // rows that one CTA marks at a time
-__device__ void zero_rows(const Tokens& tk, const unsigned* sorted, unsigned me, unsigned ctas, char* table,
-                          fgt_i64 row_bytes, unsigned* bits) {
-  const unsigned rows = (unsigned)tk.vocab;
+constexpr int kBlock = 16;           // rows of the table that are zeroed together
+constexpr int kFillBits = 1 << 18;   // rows that one CTA marks at a time
+
+// Rows without a token are zero: `rows` of a block, by the warps of a CTA.
+__device__ __forceinline__ void zero_row(char* p, fgt_i64 row_bytes) {
   const int lane = threadIdx.x % 32;
+  const int head = (int)((16 - ((uintptr_t)p & 15)) & 15);  // rows start on element boundaries: 2 bytes at least
+  const fgt_i64 lead = head < row_bytes ? head : row_bytes, body = (row_bytes - lead) / 16;
+  if (lane < lead / 2) reinterpret_cast<fgt_u16*>(p)[lane] = 0;
+  uint4* q = reinterpret_cast<uint4*>(p + lead);
+  for (fgt_i64 i = lane; i < body; i += 32) __stcs(q + i, make_uint4(0, 0, 0, 0));
+  const fgt_i64 tail = lead + body * 16;
+  if (lane < (row_bytes - tail) / 2) reinterpret_cast<fgt_u16*>(p + tail)[lane] = 0;
+}
+
+// Blocks of rows are dealt out to the filling CTAs in turn, since the frequent
+// tokens of a vocabulary lie together. A CTA marks the rows of its blocks that
+// occur: by reading all tokens (through L2), so it waits for nothing, or where
+// they are sorted already by searching them. Blocks below `now` are zeroed here,
+// the marks of the others are left for the CTAs that zero them beside the sums.
+__device__ void fill_rows(const Tokens& tk, const unsigned* sorted, unsigned me, unsigned ctas, char* table,
+                          fgt_i64 row_bytes, unsigned now, fgt_u16* present, unsigned* bits) {
+  const unsigned rows = (unsigned)tk.vocab;
   const fgt_i64 step = (fgt_i64)ctas * kFillBits;  // rows that one round covers over all CTAs
   // block / ctas as a product: exact for block * ctas < 2^32 (blocks of a round: ctas * 2^14, ctas <= 512)
   const unsigned inverse = (unsigned)(0x100000000ull / ctas) + 1;
-  for (fgt_i64 low = 0; low < rows; low += step) {  // low is a multiple of 16
+  for (fgt_i64 low = 0; low < rows; low += step) {  // low is a multiple of kBlock
     for (int i = threadIdx.x; i < kFillBits / 32; i += blockDim.x) bits[i] = 0;
     __syncthreads();
     if (sorted) {
       for (unsigned bit = threadIdx.x; bit < kFillBits; bit += blockDim.x) {
-        const fgt_i64 row = low + ((fgt_i64)(bit / 16) * ctas + me) * 16 + bit % 16;
+        const fgt_i64 row = low + ((fgt_i64)(bit / kBlock) * ctas + me) * kBlock + bit % kBlock;
         if (row >= rows) break;
         unsigned lo = 0, hi = tk.count;
         while (lo < hi) {
@@ -228,26 +272,23 @@ __device__ void zero_rows(const Tokens& tk, const unsigned* sorted, unsigned me,
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
           if (key[u] >= rows || key[u] < low || key[u] - low >= step) continue;
-          const unsigned block = (unsigned)(key[u] - low) / 16, turn = __umulhi(block, inverse);
+          const unsigned block = (unsigned)(key[u] - low) / kBlock, turn = __umulhi(block, inverse);
           if (block - turn * ctas != me) continue;
-          const unsigned bit = turn * 16 + key[u] % 16;
+          const unsigned bit = turn * kBlock + key[u] % kBlock;
           atomicOr(&bits[bit / 32], 1u << (bit % 32));
         }
       }
     }
     __syncthreads();
+    for (unsigned turn = threadIdx.x; turn < kFillBits / kBlock; turn += blockDim.x) {
+      const fgt_i64 block = low / kBlock + (fgt_i64)turn * ctas + me;
+      if (block * kBlock >= rows) break;
+      if (block >= now) present[block] = reinterpret_cast<fgt_u16*>(bits)[turn];
+    }
     for (unsigned bit = threadIdx.x / 32; bit < kFillBits; bit += blockDim.x / 32) {
-      const fgt_i64 row = low + ((fgt_i64)(bit / 16) * ctas + me) * 16 + bit % 16;
-      if (row >= rows) break;  // rows grow with bit
-      if (bits[bit / 32] >> (bit % 32) & 1) continue;
-      char* p = table + row * row_bytes;
-      const int head = (int)((16 - ((uintptr_t)p & 15)) & 15);  // rows start on element boundaries: 2 bytes at least
-      const fgt_i64 lead = head < row_bytes ? head : row_bytes, body = (row_bytes - lead) / 16;
-      if (lane < lead / 2) reinterpret_cast<fgt_u16*>(p)[lane] = 0;
-      uint4* q = reinterpret_cast<uint4*>(p + lead);
-      for (fgt_i64 i = lane; i < body; i += 32) __stcs(q + i, make_uint4(0, 0, 0, 0));
-      const fgt_i64 tail = lead + body * 16;
-      if (lane < (row_bytes - tail) / 2) reinterpret_cast<fgt_u16*>(p + tail)[lane] = 0;
+      const fgt_i64 row = low + ((fgt_i64)(bit / kBlock) * ctas + me) * kBlock + bit % kBlock;
+      if (row >= rows || row >= (fgt_i64)now * kBlock) break;  // rows grow with bit
+      if (!(bits[bit / 32] >> (bit % 32) & 1)) zero_row(table + row * row_bytes, row_bytes);
     }
     __syncthreads();
   }
@@ -255,13 +296,14 @@ __device__ void zero_rows(const Tokens& tk, const unsigned* sorted, unsigned me,
 
 // One launch does three things at once: the first cluster sorts up to
 // kSortThreads * E pairs per CTA in its distributed shared memory, the other
-// CTAs zero the table's rows that no token names, and all of them clear the
-// counters that the sums use. (With sorting = 0 the tokens are sorted already.)
+// CTAs mark the table's rows that a token names and zero part of the rest, and
+// all of them clear the counters that the sums use. (With sorting = 0 the
+// tokens are sorted already.)
 template <int E>
 __global__ void __launch_bounds__(kSortThreads, 1)
     embedding_grad_sort(Tokens tk, const unsigned* sorted, int sorting, int digit_bits, int passes, Sums out,
                         unsigned* keys, unsigned* pos, unsigned* first, fgt_i64 counters, char* table,
-                        fgt_i64 row_bytes) {
+                        fgt_i64 row_bytes, unsigned now) {
   extern __shared__ uint4 shared[];
   constexpr unsigned kPairs = kSortThreads * E;
   grid_wait();
@@ -269,17 +311,18 @@ __global__ void __launch_bounds__(kSortThreads, 1)
   for (fgt_i64 i = blockIdx.x * (fgt_i64)kSortThreads + threadIdx.x; i < counters; i += (fgt_i64)gridDim.x * kSortThreads)
     out.done[i] = 0;
   if (blockIdx.x >= sorting) {
-    zero_rows(tk, sorted, blockIdx.x - sorting, gridDim.x - sorting, table, row_bytes, reinterpret_cast<unsigned*>(shared));
+    fill_rows(tk, sorted, blockIdx.x - sorting, gridDim.x - sorting, table, row_bytes, now, out.present,
+              reinterpret_cast<unsigned*>(shared));
     return;
   }
   SortShared& s = *reinterpret_cast<SortShared*>(shared);
-  uint2* pairs = reinterpret_cast<uint2*>(&s + 1);
+  uint2 *pairs = reinterpret_cast<uint2*>(&s + 1), *staged = pairs + kPairs;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const unsigned cta = fgt_cluster_rank(), ctas = cluster_size();
   const unsigned own = warp * (32 * E) + lane;  // pairs own + 32 e: a warp's are consecutive
+  const unsigned mask = (1u << digit_bits) - 1;
   for (int pass = 0; pass < passes; ++pass) {
     const int shift = pass * digit_bits;
-    const unsigned mask = (1u << digit_bits) - 1;
     uint2 pair[E];
     unsigned digit[E], rank[E];
 #pragma unroll
@@ -292,24 +335,27 @@ __global__ void __launch_bounds__(kSortThreads, 1)
       }
       digit[e] = pair[e].x >> shift & mask;
     }
-    rank_digits<E>(s, digit_bits, digit, rank);
+    rank_digits<E>(s, digit, rank);
     scan_warps(s);
     fgt_cluster_sync();  // every CTA's totals are there, and every pair is in registers
-    unsigned all = 0, before = 0;
-    if (threadIdx.x < kDigits)
-      for (unsigned c = 0; c < ctas; ++c) {
-        const unsigned n = fgt_dsmem_ld(&s.total[threadIdx.x], c);
-        all += n;
-        before += c < cta ? n : 0;
-      }
-    scan_digits(s, all, before);
+    unsigned of[kMostSortCtas], all = 0, before = 0;
+#pragma unroll
+    for (unsigned c = 0; c < kMostSortCtas; ++c) of[c] = threadIdx.x < kDigits && c < ctas ? fgt_dsmem_ld(&s.total[threadIdx.x], c) : 0;
+#pragma unroll
+    for (unsigned c = 0; c < kMostSortCtas; ++c) {
+      all += of[c];
+      before += c < cta ? of[c] : 0;
+    }
+    scan_digits(s, threadIdx.x < kDigits ? s.total[threadIdx.x] : 0, all, before);
+    stage_pairs<E>(s, pair, shift, mask, rank, staged);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const unsigned d = pair[e].x >> shift & mask;
-      const unsigned to = s.base[d] + s.hist[warp][d] + rank[e];
+      const unsigned i = threadIdx.x + e * kSortThreads;
+      const uint2 p = staged[i];
+      const unsigned to = i + s.delta[p.x >> shift & mask];
       unsigned at = (unsigned)__cvta_generic_to_shared(pairs + to % kPairs);
       asm volatile("mapa.shared::cluster.u32 %0, %0, %1;" : "+r"(at) : "r"(to / kPairs));
-      asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(pair[e].x), "r"(pair[e].y) : "memory");
+      asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(p.x), "r"(p.y) : "memory");
     }
     fgt_cluster_sync();
   }
@@ -339,15 +385,15 @@ __global__ void __launch_bounds__(kSortThreads, 1)
 }
 
 // Batches that exceed a cluster's shared memory: each pass is two launches, a
-// CTA's digit counts and then its scatter through global memory.
-constexpr int kWideE = 8;
-constexpr unsigned kWidePairs = kSortThreads * kWideE;
-
+// CTA's digit counts and then its scatter through global memory. A scattering
+// CTA adds up the counts of all CTAs by itself, so there are few of them where
+// the pairs are many: 2 pairs per thread up to 2^18 pairs, 8 beyond.
 __device__ __forceinline__ uint2 wide_pair(const Tokens& tk, const unsigned* keys, const unsigned* pos, unsigned i) {
   if (i >= tk.count) return make_uint2(~0u, i);
   return keys ? make_uint2(keys[i], pos[i]) : make_uint2(tk.key(i), i);
 }
 
+template <int E>
 __global__ void __launch_bounds__(kSortThreads)
     embedding_grad_count(Tokens tk, const unsigned* keys, const unsigned* pos, int shift, unsigned mask, unsigned* totals) {
   __shared__ unsigned n[kDigits];
@@ -355,44 +401,51 @@ __global__ void __launch_bounds__(kSortThreads)
   grid_release();
   if (threadIdx.x < kDigits) n[threadIdx.x] = 0;
   __syncthreads();
-  for (int e = 0; e < kWideE; ++e)
-    atomicAdd(&n[wide_pair(tk, keys, pos, blockIdx.x * kWidePairs + e * kSortThreads + threadIdx.x).x >> shift & mask], 1u);
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    atomicAdd(&n[wide_pair(tk, keys, pos, (blockIdx.x * E + e) * kSortThreads + threadIdx.x).x >> shift & mask], 1u);
   __syncthreads();
   if (threadIdx.x < kDigits) totals[(fgt_i64)blockIdx.x * kDigits + threadIdx.x] = n[threadIdx.x];
 }
 
+template <int E>
 __global__ void __launch_bounds__(kSortThreads, 1)
     embedding_grad_scatter(Tokens tk, const unsigned* keys, const unsigned* pos, int shift, unsigned mask,
                            const unsigned* totals, unsigned* keys_out, unsigned* pos_out) {
   extern __shared__ uint4 shared[];
   SortShared& s = *reinterpret_cast<SortShared*>(shared);
+  uint2* staged = reinterpret_cast<uint2*>(&s + 1);
   grid_wait();
   grid_release();
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  uint2 pair[kWideE];
-  unsigned digit[kWideE], rank[kWideE];
+  uint2 pair[E];
+  unsigned digit[E], rank[E];
 #pragma unroll
-  for (int e = 0; e < kWideE; ++e) {
-    pair[e] = wide_pair(tk, keys, pos, blockIdx.x * kWidePairs + warp * (32 * kWideE) + 32 * e + lane);
+  for (int e = 0; e < E; ++e) {
+    pair[e] = wide_pair(tk, keys, pos, blockIdx.x * (kSortThreads * E) + warp * (32 * E) + 32 * e + lane);
     digit[e] = pair[e].x >> shift & mask;
   }
-  rank_digits<kWideE>(s, __popc(mask), digit, rank);
+  rank_digits<E>(s, digit, rank);
   scan_warps(s);
   unsigned all = 0, before = 0;
-  if (threadIdx.x < kDigits)
+  if (threadIdx.x < kDigits) {
+#pragma unroll 16
     for (unsigned c = 0; c < gridDim.x; ++c) {
       const unsigned n = totals[(fgt_i64)c * kDigits + threadIdx.x];
       all += n;
       before += c < blockIdx.x ? n : 0;
     }
-  scan_digits(s, all, before);
+  }
+  scan_digits(s, threadIdx.x < kDigits ? s.total[threadIdx.x] : 0, all, before);
+  stage_pairs<E>(s, pair, shift, mask, rank, staged);
 #pragma unroll
-  for (int e = 0; e < kWideE; ++e) {
-    const unsigned d = pair[e].x >> shift & mask;
-    const unsigned to = s.base[d] + s.hist[warp][d] + rank[e];
+  for (int e = 0; e < E; ++e) {
+    const unsigned i = threadIdx.x + e * kSortThreads;
+    const uint2 p = staged[i];
+    const unsigned to = i + s.delta[p.x >> shift & mask];
     if (to >= tk.count) continue;  // slots past the end
-    keys_out[to] = pair[e].x;
-    pos_out[to] = pair[e].y;
+    keys_out[to] = p.x;
+    pos_out[to] = p.y;
   }
 }
 
@@ -526,12 +579,21 @@ template <class T, bool kVec> struct Walk {
 template <class T, bool kVec>
 __global__ void __launch_bounds__(kSumThreads)
     embedding_grad_sums(Sums s, const typename T::S* __restrict__ dy, typename T::S* __restrict__ table, fgt_i64 dim,
-                        fgt_i64 chunks, float scale) {
+                        fgt_i64 chunks, float scale, unsigned summing, unsigned filled) {
   __shared__ unsigned s_pos[kSumThreads / 32][kWindow], s_key[kSumThreads / 32][kWindow];
   constexpr int N = Vec<T>::kN;
   grid_wait();
   grid_release();
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (blockIdx.x >= summing) {  // the rows that the sort's launch left: a block of rows per CTA
+    const unsigned block = filled + (blockIdx.x - summing), marks = s.present[block];
+    const fgt_i64 row_bytes = dim * (fgt_i64)sizeof(typename T::S);
+    for (int k = warp; k < kBlock; k += kSumThreads / 32) {
+      const fgt_i64 row = (fgt_i64)block * kBlock + k;
+      if (row < s.vocab && !(marks >> k & 1)) zero_row(reinterpret_cast<char*>(table) + row * row_bytes, row_bytes);
+    }
+    return;
+  }
   const fgt_i64 work = blockIdx.x * (fgt_i64)(kSumThreads / 32) + warp;
   const fgt_i64 tile = work / chunks, chunk = work % chunks;
   if (tile >= s.tiles) return;
@@ -610,20 +672,23 @@ void check(const fgt_embedding_desc* d) {
 
 // How the workspace of the gradient is laid out (bytes from its start).
 struct GradPlan {
-  bool wide;             // more pairs than a cluster holds
-  int64_t tiles, chunks, sort_ctas;
-  size_t keys, pos, first, done, partial, totals, keys2, pos2, bytes;
+  int wide_pairs;        // per thread of the sort through global memory (0: a cluster holds all pairs)
+  int64_t tiles, chunks, blocks, sort_ctas;
+  size_t keys, pos, first, done, present, partial, totals, keys2, pos2, bytes;
 };
+
+constexpr int64_t kClusterPairs = 8 * kSortThreads * kMostSortCtas;
 
 GradPlan plan_grad(const fgt_embedding_desc* d) {
   check(d);
   require(d->vocab < 0xfffffffell, "the gradient takes a vocabulary below 2^32 - 2");
-  require(d->count < 0x7fffffffll - kWidePairs, "the gradient takes fewer than 2^31 - 2^14 indices");
+  require(d->count < 0x7fffffffll - 8 * kSortThreads, "the gradient takes fewer than 2^31 - 2^13 indices");
   GradPlan p{};
   const int64_t per_chunk = 32 * (16 / dtype_size(d->dtype));
-  p.wide = d->count > kSortCtas * kSortThreads * 16;
+  p.wide_pairs = d->count <= kClusterPairs ? 0 : d->count <= 1 << 18 ? 2 : 8;
   p.tiles = (d->count + kTile - 1) / kTile;
   p.chunks = (d->dim + per_chunk - 1) / per_chunk;
+  p.blocks = (d->vocab + kBlock - 1) / kBlock;
   size_t at = 0;
   auto take = [&](int64_t bytes) {
     const size_t here = at;
@@ -634,9 +699,10 @@ GradPlan plan_grad(const fgt_embedding_desc* d) {
   p.pos = take(d->count * 4);
   p.first = take(p.tiles * 4);
   p.done = take(p.tiles * p.chunks * 8);
+  p.present = take(p.blocks * 2);
   p.partial = take(d->count > kPiece ? 2 * p.tiles * d->dim * 4 : 0);  // a run has a second piece at most
-  if (p.wide) {
-    p.sort_ctas = (d->count + kWidePairs - 1) / kWidePairs;
+  if (p.wide_pairs) {
+    p.sort_ctas = (d->count + kSortThreads * p.wide_pairs - 1) / (kSortThreads * p.wide_pairs);
     p.totals = take(p.sort_ctas * kDigits * 4);
     p.keys2 = take(d->count * 4);
     p.pos2 = take(d->count * 4);
@@ -696,23 +762,31 @@ extern "C" fgt_status fgt_embedding_grad(const fgt_embedding_desc* d, const void
     const Launch l{(cudaStream_t)stream, programmatic((cudaStream_t)stream)};
     const Tokens tk{Index{indices, d->index_dtype == FGT_I64}, (unsigned)d->count, d->vocab, d->padding_index};
     unsigned *keys = (unsigned*)(ws + p.keys), *pos = (unsigned*)(ws + p.pos), *first = (unsigned*)(ws + p.first);
-    const Sums s{keys, pos, first, (unsigned long long*)(ws + p.done), (float*)(ws + p.partial),
+    const Sums s{keys, pos, first, (unsigned long long*)(ws + p.done), (float*)(ws + p.partial), (fgt_u16*)(ws + p.present),
                  (unsigned)d->count, (unsigned)p.tiles, (unsigned)d->vocab};
     int bits = 1;
     while (d->vocab >> bits) ++bits;  // of the largest key, which is vocab itself
-    const int passes = (bits + 8) / 9, digit_bits = (bits + passes - 1) / passes;
+    const int passes = (bits + kDigitBits - 1) / kDigitBits, digit_bits = (bits + passes - 1) / passes;
     const int64_t row_bytes = d->dim * dtype_size(d->dtype);
 
-    // the sort, beside CTAs that zero rows
-    auto sort = [&](auto kernel, int pairs_per_thread, unsigned cluster, int sorting) {
-      size_t smem = sorting ? sizeof(SortShared) + (size_t)kSortThreads * pairs_per_thread * sizeof(uint2) : 0;
+    // The sort, beside CTAs that zero as many rows as take about its time
+    // (4 MB/us: what is left of the GPU writes 5 to 6); the rest is zeroed
+    // beside the sums. With sorting = 0 all of it is.
+    unsigned now = 0;
+    auto sort = [&](auto kernel, int pairs, unsigned cluster, int sorting) {
+      size_t smem = sorting ? sizeof(SortShared) + (size_t)kSortThreads * pairs * 2 * sizeof(uint2) : 0;
       smem = std::max(smem, (size_t)kFillBits / 8);
-      // as many clusters as run at once: a GPC's SMs do not all fit clusters of 8
+      // as many clusters as run at once: a GPC's SMs do not all fit clusters of 8 or 16
       const unsigned grid = std::max(2u, active_clusters(kernel, kSortThreads, smem, cluster)) * cluster;
-      launch(l, kernel, grid, kSortThreads, smem, cluster, tk, p.wide ? keys : nullptr, sorting, digit_bits, passes, s, keys, pos, first,
-             p.tiles * p.chunks, (char*)dtable, row_bytes);
+      if (sorting) now = (unsigned)std::min<int64_t>(p.blocks, (int64_t)(passes * (2 + 1.5 * pairs) + 3) * 4000000 / (row_bytes * kBlock));
+      if (d->count == 0) now = (unsigned)p.blocks;
+      launch(l, kernel, grid, kSortThreads, smem, cluster, tk, p.wide_pairs ? keys : nullptr, sorting, digit_bits, passes, s,
+             keys, pos, first, p.tiles * p.chunks, (char*)dtable, row_bytes, now);
     };
-    if (p.wide) {
+    auto wide = [&](auto pairs) {
+      constexpr int E = decltype(pairs)::value;
+      const size_t smem = sizeof(SortShared) + kSortThreads * E * sizeof(uint2);
+      active_clusters(embedding_grad_scatter<E>, kSortThreads, smem, 1);  // leave for the shared memory
       unsigned *from_k = nullptr, *from_p = nullptr;
       for (int pass = 0; pass < passes; ++pass) {
         const bool back = (passes - 1 - pass) % 2 == 1;  // the last pass writes keys and pos
@@ -720,34 +794,41 @@ extern "C" fgt_status fgt_embedding_grad(const fgt_embedding_desc* d, const void
         unsigned* totals = (unsigned*)(ws + p.totals);
         const int shift = pass * digit_bits;
         const unsigned mask = (1u << digit_bits) - 1;
-        launch(l, embedding_grad_count, (unsigned)p.sort_ctas, kSortThreads, 0, 1, tk, from_k, from_p, shift, mask, totals);
-        launch(l, embedding_grad_scatter, (unsigned)p.sort_ctas, kSortThreads, sizeof(SortShared), 1, tk, from_k, from_p,
-               shift, mask, totals, to_k, to_p);
+        launch(l, embedding_grad_count<E>, (unsigned)p.sort_ctas, kSortThreads, 0, 1, tk, from_k, from_p, shift, mask, totals);
+        launch(l, embedding_grad_scatter<E>, (unsigned)p.sort_ctas, kSortThreads, smem, 1, tk, from_k, from_p, shift, mask,
+               totals, to_k, to_p);
         from_k = to_k;
         from_p = to_p;
       }
       launch(l, embedding_grad_first, blocks_for(p.tiles, 256, "indices"), 256, 0, 1, keys, (unsigned)d->count, first);
       sort(embedding_grad_sort<1>, 1, 1, 0);
+    };
+    if (p.wide_pairs == 2) {
+      wide(std::integral_constant<int, 2>{});
+    } else if (p.wide_pairs == 8) {
+      wide(std::integral_constant<int, 8>{});
     } else if (d->count <= kSortThreads) {
       sort(embedding_grad_sort<1>, 1, 1, d->count > 0);
     } else if (d->count <= kSortCtas * kSortThreads) {
       sort(embedding_grad_sort<1>, 1, kSortCtas, kSortCtas);
-    } else if (d->count <= kSortCtas * kSortThreads * 2) {
-      sort(embedding_grad_sort<2>, 2, kSortCtas, kSortCtas);
-    } else if (d->count <= kSortCtas * kSortThreads * 4) {
-      sort(embedding_grad_sort<4>, 4, kSortCtas, kSortCtas);
-    } else if (d->count <= kSortCtas * kSortThreads * 8) {
-      sort(embedding_grad_sort<8>, 8, kSortCtas, kSortCtas);
+    } else if (d->count <= kMostSortCtas * kSortThreads) {
+      sort(embedding_grad_sort<1>, 1, kMostSortCtas, kMostSortCtas);
+    } else if (d->count <= kMostSortCtas * kSortThreads * 2) {
+      sort(embedding_grad_sort<2>, 2, kMostSortCtas, kMostSortCtas);
+    } else if (d->count <= kMostSortCtas * kSortThreads * 4) {
+      sort(embedding_grad_sort<4>, 4, kMostSortCtas, kMostSortCtas);
     } else {
-      sort(embedding_grad_sort<16>, 16, kSortCtas, kSortCtas);
+      sort(embedding_grad_sort<8>, 8, kMostSortCtas, kMostSortCtas);
     }
     if (d->count == 0) return;
-    const unsigned grid = blocks_for(p.tiles * p.chunks, kSumThreads / 32, "indices x dim");
+    const unsigned summing = blocks_for(p.tiles * p.chunks, kSumThreads / 32, "indices x dim");
+    const unsigned filling = (unsigned)(p.blocks - now);
+    require((int64_t)summing + filling <= 0x7fffffff, "indices x dim and vocab are too large for one launch");
     for_dtype(d->dtype, [&](auto t) {
       using T = decltype(t);
       using S = typename T::S;
       auto kernel = d->dim % Vec<T>::kN == 0 ? embedding_grad_sums<T, true> : embedding_grad_sums<T, false>;
-      launch(l, kernel, grid, kSumThreads, 0, 1, s, (const S*)dy, (S*)dtable, d->dim, p.chunks, d->scale);
+      launch(l, kernel, summing + filling, kSumThreads, 0, 1, s, (const S*)dy, (S*)dtable, d->dim, p.chunks, d->scale, summing, now);
     });
   });
 }

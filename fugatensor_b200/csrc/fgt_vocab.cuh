@@ -225,6 +225,7 @@ template <class K> unsigned active_clusters(K kernel, unsigned threads, size_t s
       cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "cudaFuncSetAttribute");
       most = smem;
     }
+    if (cluster > 8) cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "cudaFuncSetAttribute");
     int c = 0;
     if (cluster == 1) {
       cuda_check(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&c, kernel, (int)threads, smem), "cudaOccupancyMaxActiveBlocksPerMultiprocessor");
