@@ -90,12 +90,13 @@ __global__ void __launch_bounds__(kLookupThreads)
 // the token, or V for tokens that have no gradient (outside the table, the
 // padding row): those end up last. Digits have at most 9 bits, so a vocabulary
 // below 2^18 takes two passes. A CTA holds kSortThreads * E pairs in shared
-// memory; each warp ranks its pairs 32 at a time (the lanes with the same
-// digit are found by one ballot per bit: match.any walks the distinct values
-// and took 2 us for a round of 32 warps), and the warps' counts are summed per
-// digit. A pass puts the CTA's pairs in order before it sends them on, so that
-// what goes to another CTA goes in runs (sent singly, a pass over 8 pairs per
-// thread spent 10,000 cycles on it).
+// memory; each warp ranks its pairs 32 at a time, and the warps' counts are
+// summed per digit. The lanes with the same digit find each other in a table
+// of lane masks per warp and digit (a round of 32 warps took 2 us with
+// match.any, which walks the distinct values, 0.5 us with a ballot per bit). A
+// pass puts the CTA's pairs in order before it sends them on, so that what goes
+// to another CTA goes in runs (sent singly, a pass over 8 pairs per thread
+// spent 10,000 cycles on it).
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
 constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits;
 constexpr int kSortCtas = 8, kMostSortCtas = 16;  // the largest portable cluster, the largest
@@ -105,8 +106,13 @@ struct Tokens {
   unsigned count;
   fgt_i64 vocab, padding;
   __device__ __forceinline__ unsigned key(unsigned i) const {
-    const fgt_i64 t = ids[i];
-    return t >= 0 && t < vocab && t != padding ? (unsigned)t : (unsigned)vocab;
+    const unsigned none = (unsigned)vocab, skip = (unsigned)padding;
+    if (ids.wide) {
+      const fgt_i64 t = static_cast<const fgt_i64*>(ids.p)[i];
+      return t >= 0 && t < vocab && t != padding ? (unsigned)t : none;
+    }
+    const int t = static_cast<const int*>(ids.p)[i];
+    return t >= 0 && (unsigned)t < none && (unsigned)t != skip ? (unsigned)t : none;
   }
 };
 
@@ -115,31 +121,32 @@ struct SortShared {
   unsigned total[kDigits];                   // per digit: the CTA's count
   unsigned start[kDigits];                   // per digit: its first place in the CTA
   unsigned delta[kDigits];                   // per digit: from a place in the CTA to one among all pairs
+  unsigned totals[kMostSortCtas][kDigits];   // every CTA's total
   unsigned warp_sum[2][kDigits / 32];
 };
 
 // Stable rank of each of a warp's E x 32 digits within the warp; hist[warp]
-// ends as the warp's counts.
-template <int E> __device__ __forceinline__ void rank_digits(SortShared& s, const unsigned (&digit)[E], unsigned (&rank)[E]) {
+// ends as the warp's counts. `masks` is scratch: kSortWarps x kDigits words.
+constexpr size_t kMaskBytes = (size_t)kSortWarps * kDigits * 4;
+template <int E>
+__device__ __forceinline__ void rank_digits(SortShared& s, const unsigned (&digit)[E], unsigned (&rank)[E], unsigned* masks) {
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  for (int d = lane; d < kDigits; d += 32) s.hist[warp][d] = 0;
+  unsigned* const mask = masks + warp * kDigits;
+  for (int d = lane; d < kDigits / 4; d += 32) reinterpret_cast<uint4*>(mask)[d] = make_uint4(0, 0, 0, 0);
+  for (int d = lane; d < kDigits / 8; d += 32) reinterpret_cast<uint4*>(s.hist[warp])[d] = make_uint4(0, 0, 0, 0);
   __syncwarp();
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    unsigned same = ~0u;
-#pragma unroll
-    for (int b = 0; b < kDigitBits; ++b) {
-      const unsigned set = __ballot_sync(~0u, digit[e] >> b & 1);
-      same &= digit[e] >> b & 1 ? set : ~set;
-    }
-    const int leader = __ffs(same) - 1;
-    unsigned before = 0;
-    if (lane == leader) {
-      before = s.hist[warp][digit[e]];
+    atomicOr(&mask[digit[e]], 1u << lane);
+    __syncwarp();
+    const unsigned same = mask[digit[e]], before = s.hist[warp][digit[e]];
+    rank[e] = before + __popc(same & ((1u << lane) - 1));
+    __syncwarp();
+    if (same >> lane == 1u) {  // the last of them
       s.hist[warp][digit[e]] = (unsigned short)(before + __popc(same));
+      mask[digit[e]] = 0;
     }
     __syncwarp();
-    rank[e] = __shfl_sync(~0u, before, leader) + __popc(same & ((1u << lane) - 1));
   }
 }
 
@@ -236,19 +243,23 @@ __device__ __forceinline__ void zero_row(char* p, fgt_i64 row_bytes) {
 }
 
 // Blocks of rows are dealt out to the filling CTAs in turn, since the frequent
-// tokens of a vocabulary lie together. A CTA marks the rows of its blocks that
-// occur: by reading all tokens (through L2), so it waits for nothing, or where
-// they are sorted already by searching them. Blocks below `now` are zeroed here,
-// the marks of the others are left for the CTAs that zero them beside the sums.
+// tokens of a vocabulary lie together. The CTAs of a cluster mark the rows of
+// their blocks that occur: they share out the tokens, and each marks what it
+// finds in the owner's shared memory, so they wait for nothing but each other
+// (every CTA reading all 65536 tokens by itself took 17 us, all that time on L2).
+// Where the tokens are sorted already they are searched instead. Blocks below
+// `now` are zeroed here, the marks of the others are left for the CTAs that zero
+// them beside the sums.
 __device__ void fill_rows(const Tokens& tk, const unsigned* sorted, unsigned me, unsigned ctas, char* table,
                           fgt_i64 row_bytes, unsigned now, fgt_u16* present, unsigned* bits) {
   const unsigned rows = (unsigned)tk.vocab;
+  const unsigned mates = cluster_size(), rank = fgt_cluster_rank(), leader = me - rank;  // this cluster: CTAs [leader, leader + mates)
   const fgt_i64 step = (fgt_i64)ctas * kFillBits;  // rows that one round covers over all CTAs
   // block / ctas as a product: exact for block * ctas < 2^32 (blocks of a round: ctas * 2^14, ctas <= 512)
   const unsigned inverse = (unsigned)(0x100000000ull / ctas) + 1;
   for (fgt_i64 low = 0; low < rows; low += step) {  // low is a multiple of kBlock
     for (int i = threadIdx.x; i < kFillBits / 32; i += blockDim.x) bits[i] = 0;
-    __syncthreads();
+    fgt_cluster_sync();
     if (sorted) {
       for (unsigned bit = threadIdx.x; bit < kFillBits; bit += blockDim.x) {
         const fgt_i64 row = low + ((fgt_i64)(bit / kBlock) * ctas + me) * kBlock + bit % kBlock;
@@ -264,22 +275,26 @@ __device__ void fill_rows(const Tokens& tk, const unsigned* sorted, unsigned me,
         if (lo < tk.count && sorted[lo] == row) atomicOr(&bits[bit / 32], 1u << (bit % 32));
       }
     } else {
-      constexpr int kBatch = 16;  // loads in flight per thread
-      for (unsigned i = threadIdx.x; i < tk.count; i += kBatch * blockDim.x) {
+      constexpr int kBatch = 8;  // loads in flight per thread
+      const unsigned span = (unsigned)min(step, rows - low), from = (unsigned)low, stride = mates * blockDim.x;
+      const unsigned here = (unsigned)__cvta_generic_to_shared(bits);
+      for (unsigned i = rank * blockDim.x + threadIdx.x; i < tk.count; i += kBatch * stride) {
         unsigned key[kBatch];
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) key[u] = i + u * blockDim.x < tk.count ? tk.key(i + u * blockDim.x) : rows;
+        for (int u = 0; u < kBatch; ++u) key[u] = i + u * stride < tk.count ? tk.key(i + u * stride) : rows;
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
-          if (key[u] >= rows || key[u] < low || key[u] - low >= step) continue;
-          const unsigned block = (unsigned)(key[u] - low) / kBlock, turn = __umulhi(block, inverse);
-          if (block - turn * ctas != me) continue;
-          const unsigned bit = turn * kBlock + key[u] % kBlock;
-          atomicOr(&bits[bit / 32], 1u << (bit % 32));
+          const unsigned at = key[u] - from, block = at / kBlock, turn = __umulhi(block, inverse);
+          const unsigned mate = block - turn * ctas - leader;  // of this cluster, if it is below mates
+          if (at >= span || mate >= mates) continue;           // (a key below `from` wraps past span)
+          const unsigned bit = turn * kBlock + at % kBlock;
+          unsigned to;
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(here + bit / 32 * 4), "r"(mate));
+          asm volatile("red.relaxed.cluster.shared::cluster.or.b32 [%0], %1;" ::"r"(to), "r"(1u << (bit % 32)) : "memory");
         }
       }
     }
-    __syncthreads();
+    fgt_cluster_sync();
     for (unsigned turn = threadIdx.x; turn < kFillBits / kBlock; turn += blockDim.x) {
       const fgt_i64 block = low / kBlock + (fgt_i64)turn * ctas + me;
       if (block * kBlock >= rows) break;
@@ -316,7 +331,8 @@ __global__ void __launch_bounds__(kSortThreads, 1)
     return;
   }
   SortShared& s = *reinterpret_cast<SortShared*>(shared);
-  uint2 *pairs = reinterpret_cast<uint2*>(&s + 1), *staged = pairs + kPairs;
+  uint2 *pairs = reinterpret_cast<uint2*>(&s + 1), *staged = pairs + kPairs;  // staged: the masks' scratch too
+  if (cluster_size() > 1) fgt_cluster_sync();  // every CTA has started before another writes to it
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const unsigned cta = fgt_cluster_rank(), ctas = cluster_size();
   const unsigned own = warp * (32 * E) + lane;  // pairs own + 32 e: a warp's are consecutive
@@ -335,18 +351,26 @@ __global__ void __launch_bounds__(kSortThreads, 1)
       }
       digit[e] = pair[e].x >> shift & mask;
     }
-    rank_digits<E>(s, digit, rank);
+    rank_digits<E>(s, digit, rank, reinterpret_cast<unsigned*>(staged));
     scan_warps(s);
-    fgt_cluster_sync();  // every CTA's totals are there, and every pair is in registers
-    unsigned of[kMostSortCtas], all = 0, before = 0;
-#pragma unroll
-    for (unsigned c = 0; c < kMostSortCtas; ++c) of[c] = threadIdx.x < kDigits && c < ctas ? fgt_dsmem_ld(&s.total[threadIdx.x], c) : 0;
-#pragma unroll
-    for (unsigned c = 0; c < kMostSortCtas; ++c) {
-      all += of[c];
-      before += c < cta ? of[c] : 0;
+    const unsigned total = threadIdx.x < kDigits ? s.total[threadIdx.x] : 0;
+    if (threadIdx.x < kDigits) {
+      const unsigned at = (unsigned)__cvta_generic_to_shared(&s.totals[cta][threadIdx.x]);
+      for (unsigned c = 0; c < ctas; ++c) {
+        unsigned to;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(at), "r"(c));
+        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to), "r"(total) : "memory");
+      }
     }
-    scan_digits(s, threadIdx.x < kDigits ? s.total[threadIdx.x] : 0, all, before);
+    fgt_cluster_sync();  // every CTA's totals are there, and every pair is in registers
+    unsigned all = 0, before = 0;
+    if (threadIdx.x < kDigits)
+      for (unsigned c = 0; c < ctas; ++c) {
+        const unsigned n = s.totals[c][threadIdx.x];
+        all += n;
+        before += c < cta ? n : 0;
+      }
+    scan_digits(s, total, all, before);
     stage_pairs<E>(s, pair, shift, mask, rank, staged);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -425,7 +449,7 @@ __global__ void __launch_bounds__(kSortThreads, 1)
     pair[e] = wide_pair(tk, keys, pos, blockIdx.x * (kSortThreads * E) + warp * (32 * E) + 32 * e + lane);
     digit[e] = pair[e].x >> shift & mask;
   }
-  rank_digits<E>(s, digit, rank);
+  rank_digits<E>(s, digit, rank, reinterpret_cast<unsigned*>(staged));
   scan_warps(s);
   unsigned all = 0, before = 0;
   if (threadIdx.x < kDigits) {
@@ -774,18 +798,19 @@ extern "C" fgt_status fgt_embedding_grad(const fgt_embedding_desc* d, const void
     // beside the sums. With sorting = 0 all of it is.
     unsigned now = 0;
     auto sort = [&](auto kernel, int pairs, unsigned cluster, int sorting) {
-      size_t smem = sorting ? sizeof(SortShared) + (size_t)kSortThreads * pairs * 2 * sizeof(uint2) : 0;
+      const size_t held = (size_t)kSortThreads * pairs * sizeof(uint2);
+      size_t smem = sorting ? sizeof(SortShared) + held + std::max(held, kMaskBytes) : 0;
       smem = std::max(smem, (size_t)kFillBits / 8);
       // as many clusters as run at once: a GPC's SMs do not all fit clusters of 8 or 16
       const unsigned grid = std::max(2u, active_clusters(kernel, kSortThreads, smem, cluster)) * cluster;
-      if (sorting) now = (unsigned)std::min<int64_t>(p.blocks, (int64_t)(passes * (2 + 1.5 * pairs) + 3) * 4000000 / (row_bytes * kBlock));
+      if (sorting) now = (unsigned)std::min<int64_t>(p.blocks, (int64_t)(passes * (5 + 1.2 * pairs) + 3) * 4000000 / (row_bytes * kBlock));
       if (d->count == 0) now = (unsigned)p.blocks;
       launch(l, kernel, grid, kSortThreads, smem, cluster, tk, p.wide_pairs ? keys : nullptr, sorting, digit_bits, passes, s,
              keys, pos, first, p.tiles * p.chunks, (char*)dtable, row_bytes, now);
     };
     auto wide = [&](auto pairs) {
       constexpr int E = decltype(pairs)::value;
-      const size_t smem = sizeof(SortShared) + kSortThreads * E * sizeof(uint2);
+      const size_t smem = sizeof(SortShared) + std::max(kSortThreads * E * sizeof(uint2), kMaskBytes);
       active_clusters(embedding_grad_scatter<E>, kSortThreads, smem, 1);  // leave for the shared memory
       unsigned *from_k = nullptr, *from_p = nullptr;
       for (int pass = 0; pass < passes; ++pass) {
