@@ -150,13 +150,13 @@ struct Stat {
 };
 
 // The statistics of a warp's lanes joined; every lane gets the result.
-__device__ __forceinline__ Stat warp_join(Stat a, bool whole) {
+template <bool kAll> __device__ __forceinline__ Stat warp_join(Stat a, bool whole) {
   const float c = fgt_redux_max(a.c), d = __fsub_rn(a.c, c == kNegInf ? 0.0f : c);
   float s = __fmul_rn(a.s, fgt_ex2_approx(whole ? d : __fmul_rn(d, kLog2e)));
 #pragma unroll
   for (int k = 16; k; k >>= 1) {
     s += __shfl_xor_sync(~0u, s, k);
-    a.all += __shfl_xor_sync(~0u, a.all, k);
+    if (kAll) a.all += __shfl_xor_sync(~0u, a.all, k);
   }
   return Stat{c, s, a.all};
 }
@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
       const float2 both_sums = __fadd2_rn(sum[0], sum[1]);
       stat.s = both_sums.x + both_sums.y;
       stat.all = all.x + all.y;
-      stat = warp_join(stat, whole);
+      stat = warp_join<kAll>(stat, whole);
       if (G != kWarp) {
         Stat* slot = &s_stat[parity][cta * warps + warp];
         if (G == kCluster) {
@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
           total.s += o.s * fgt_ex2_approx(whole ? d : d * kLog2e);
           total.all += o.all;
         }
-        stat = warp_join(total, whole);
+        stat = warp_join<kAll>(total, whole);
         parity ^= 1;  // the next exchange's writers do not meet this one's readers
       }
       if (!whole || (stat.s > 0.0f && stat.s < __int_as_float(0x7f800000))) break;  // the same decision for the whole group
@@ -363,14 +363,17 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
       }
     }
 
-    const float g = now.g, lse = whole ? (stat.c + log2f(stat.s)) * kLn2 : stat.c + logf(stat.s);
-    if (losses && cta == 0 && me == 0) {
+    const bool tells = losses && cta == 0 && me == 0;
+    float lse = 0.0f;  // for the thread that stores the loss, and for all where it is part of the gradient
+    if (tells || r.z != 0.0f) lse = whole ? (stat.c + log2f(stat.s)) * kLn2 : stat.c + logf(stat.s);
+    if (tells) {
       float l = lse - (1.0f - r.smoothing) * now.x_t;
       if (kAll) l -= r.smoothing / (float)r.vocab * stat.all;
       if (r.z != 0.0f) l += r.z * lse * lse;
       losses[row] = l;
     }
     if (!dlogits) continue;
+    const float g = now.g;
     const float peak = g * (r.z != 0.0f ? 1.0f + 2.0f * r.z * lse : 1.0f) / stat.s, share = g * (r.smoothing / (float)r.vocab);
     const int in_vecs = (int)now.t - now.lead, hit = in_vecs >= 0 ? in_vecs / N : -1;  // the vector that holds the target
     auto gradient = [&](auto exp2) {

@@ -243,7 +243,7 @@ class Engine:
         import torch
         from . import operators
         device = self._cuda_device()
-        index, known, ran = device.index, {}, []
+        index, known, ran, kept = device.index, {}, [], []
         self.last_execution_plan = self.last_report = None
 
         def data(t):
@@ -252,6 +252,9 @@ class Engine:
                 x = x.to(device)
             if not x.is_contiguous():
                 raise ValueError(f"operand must be a contiguous CUDA tensor, got {x.dtype}{list(x.shape)} with strides {x.stride()}")
+            if x.data_ptr() % 16:  # a slice (ids[1:]): the entry points take 16-byte aligned buffers
+                x = x.clone()
+                kept.append(x)
             return x
 
         def partition(wanted):

@@ -373,6 +373,16 @@ def test_on_another_stream_and_in_a_cuda_graph():
         assert all(torch.equal(a, b) for a, b in zip(held, want))
 
 
+def test_slices_that_are_not_aligned():
+    """Inputs and targets are commonly one buffer, a token apart."""
+    text = torch.tensor([3, 1, 4, 1, 5, 0, 2, 6], device="cuda")
+    table = torch.arange(7.0 * 7, device="cuda").reshape(7, 7)
+    y = F.embedding(R.wrap(table), R.wrap(text[:-1]))
+    l = F.cross_entropy(y, R.wrap(text[1:]), reduction="none")
+    loss, lbound, _, _ = R.cross_entropy(table[text[:-1]], text[1:], reduction="none")
+    R.check(l.torch(), loss, lbound)
+
+
 def test_evaluate_host_downloads_operator_results():
     x = torch.randn(4, 50, device="cuda")
     t = torch.tensor([1, 2, 3, 4], device="cuda")
@@ -381,3 +391,18 @@ def test_evaluate_host_downloads_operator_results():
     assert not l.torch().is_cuda
     loss, lbound, _, _ = R.cross_entropy(x, t, reduction="none")
     R.check(l.torch(), loss.cpu(), lbound.cpu())
+
+
+def test_bigram_example_learns_and_generates():
+    import importlib.util
+    from pathlib import Path
+    path = Path(__file__).resolve().parent.parent / "examples" / "bigram.py"
+    spec = importlib.util.spec_from_file_location("bigram", path)
+    bigram = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(bigram)
+    text = b"abracadabra, " * 200
+    table, losses = bigram.train(text, steps=30, batch=512, rate=20.0)
+    assert abs(losses[0] - math.log(256)) < 1e-2 and losses[-1] < 1.0  # lse^2 of the first step: 1e-4 * 30.7
+    lines = bigram.generate(table, b"ab", sequences=3, length=20, allowed=b"abcdr, ")
+    assert len(lines) == 3 and all(len(l) == 20 and set(l) <= set(b"abcdr, ") for l in lines)
+    assert lines == bigram.generate(table, b"ab", sequences=3, length=20, allowed=b"abcdr, ")
