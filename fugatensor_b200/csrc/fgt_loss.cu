@@ -192,60 +192,66 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
   // wanted, kBatch per thread at a time and kStages - 1 batches ahead.
   const int passes = dlogits ? 2 : 1;
   fgt_i64 ahead = (G == kWarp ? blockIdx.x * (fgt_i64)warps + warp : blockIdx.x / ctas) - step, t_ahead = target(ahead + step);
-  const uint4* from = nullptr;
-  int at = 0, stop = 0, pass = passes - 1, to = 0;  // [at, stop) of this pass are still to be copied
+  const uint4 *from = nullptr, *src = nullptr;  // this thread's first vector of the row, its next one
+  int part = 0, left = 0, pass = passes - 1;    // the group's vectors of the row; those still to be copied
+  constexpr unsigned kStage = kBatch * kThreads * 16;
   const unsigned mine = (unsigned)__cvta_generic_to_shared(ring + threadIdx.x);
+  unsigned slot = mine;
   auto advance = [&]() {
-    if (at >= stop && ahead < r.rows) {
-      if (++pass == passes) {
+    if (left <= 0) {
+      if (++pass < passes) {
+        src = from;
+        left = part;
+      } else {
         pass = 0;
         bool live;
         do {
           ahead += step;
+          if (ahead >= r.rows) break;
           live = r.counts(t_ahead);
           t_ahead = target(ahead + step);
           const int lead = lead_of(ahead);
-          stop = end_of(lead);
-          from = reinterpret_cast<const uint4*>(logits + ahead * r.vocab + lead) + me;
-        } while (ahead < r.rows && (!live || stop <= first));
+          part = end_of(lead) - first;
+          src = from = reinterpret_cast<const uint4*>(logits + ahead * r.vocab + lead) + (first + me);
+        } while (!live || part <= 0);
+        left = ahead < r.rows ? part : 0;
+        if (!left) pass = passes - 1;  // the rows are through
       }
-      at = first;
     }
-    if (ahead < r.rows) {
-      const unsigned slot = mine + (unsigned)(to * (kBatch * kThreads * 16));
-      const uint4* src = from + at;
-      if (at + kStep <= stop) {
+    if (left >= kStep) {
 #pragma unroll
-        for (int b = 0; b < kBatch; ++b) fgt_cp_async<16>(slot + b * kThreads * 16, src + b * threads);
-      } else {
+      for (int b = 0; b < kBatch; ++b) fgt_cp_async<16>(slot + b * kThreads * 16, src + b * threads);
+    } else {
 #pragma unroll
-        for (int b = 0; b < kBatch; ++b)
-          if (at + b * threads + me < stop) fgt_cp_async<16>(slot + b * kThreads * 16, src + b * threads);
-      }
-      at += kStep;
+      for (int b = 0; b < kBatch; ++b)
+        if (me + b * threads < left) fgt_cp_async<16>(slot + b * kThreads * 16, src + b * threads);
     }
     fgt_cp_commit();
-    to = to + 1 == kStages ? 0 : to + 1;
+    src += kStep;
+    left -= kStep;
+    slot = slot == mine + (kStages - 1) * kStage ? mine : slot + kStage;
   };
   for (int k = 0; k < kStages - 1; ++k) advance();
   int st = 0;
-  // f(vectors from `first` on, slot, vector) for this thread's vectors of a pass
-  auto each = [&](int end, auto f) {
-    for (int i = first; i < end; i += kStep) {
+  // f(slot, vector) for this thread's vectors of a pass, kBatch per turn; turn() after each
+  auto each = [&](int vectors, auto f, auto turn) {
+    for (int n = vectors; n > 0; n -= kStep) {
       advance();
       fgt_cp_wait<kStages - 1>();
       const uint4* x = ring + st * (kBatch * kThreads) + threadIdx.x;
-      if (i + kStep <= end) {
+      if (n >= kStep) {
 #pragma unroll
-        for (int b = 0; b < kBatch; ++b) f(i + me + b * threads, b, x[b * kThreads]);
+        for (int b = 0; b < kBatch; ++b) f(b, x[b * kThreads]);
       } else {
 #pragma unroll
         for (int b = 0; b < kBatch; ++b)
-          if (i + me + b * threads < end) f(i + me + b * threads, b, x[b * kThreads]);
+          if (me + b * threads < n) f(b, x[b * kThreads]);
       }
+      turn();
       st = st + 1 == kStages ? 0 : st + 1;
     }
   };
+  const float smoothed = r.smoothing / (float)r.vocab;
 
   fgt_i64 row = G == kWarp ? blockIdx.x * (fgt_i64)warps + warp : blockIdx.x / ctas;
   int parity = 0;
@@ -295,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
       sum[0] = Exponent<true>(stat.c)(make_float2(now.x_single, kNegInf));
     }
     if (now.single >= 0) all.x = now.x_single;
-    each(end, [&](int, int b, const uint4& u) {
+    each(end - first, [&](int b, const uint4& u) {
       float v[N];
       Vec<T>::unpack(u, v);
       if (stat.c == kNegInf) {
@@ -310,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
         sum[b % 2] = __fadd2_rn(sum[b % 2], exp2(make_float2(v[e], v[e + 1])));
         if (kAll) all = __fadd2_rn(all, make_float2(v[e], v[e + 1]));
       }
-    });
+    }, [] {});
     for (;; whole = false) {
       const float2 both_sums = __fadd2_rn(sum[0], sum[1]);
       stat.s = both_sums.x + both_sums.y;
@@ -368,17 +374,18 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
     if (tells || r.z != 0.0f) lse = whole ? (stat.c + log2f(stat.s)) * kLn2 : stat.c + logf(stat.s);
     if (tells) {
       float l = lse - (1.0f - r.smoothing) * now.x_t;
-      if (kAll) l -= r.smoothing / (float)r.vocab * stat.all;
+      if (kAll) l -= smoothed * stat.all;
       if (r.z != 0.0f) l += r.z * lse * lse;
       losses[row] = l;
     }
     if (!dlogits) continue;
     const float g = now.g;
-    const float peak = g * (r.z != 0.0f ? 1.0f + 2.0f * r.z * lse : 1.0f) / stat.s, share = g * (r.smoothing / (float)r.vocab);
+    const float peak = g * (r.z != 0.0f ? 1.0f + 2.0f * r.z * lse : 1.0f) / stat.s, share = g * smoothed;
     const int in_vecs = (int)now.t - now.lead, hit = in_vecs >= 0 ? in_vecs / N : -1;  // the vector that holds the target
     auto gradient = [&](auto exp2) {
       auto of = [&](float2 x) { return __ffma2_rn(exp2(x), both(peak), both(-share)); };
-      each(end, [&](int i, int, const uint4& u) {
+      uint4* o = out + (first + me);
+      each(end - first, [&](int b, const uint4& u) {
         float v[N];
         Vec<T>::unpack(u, v);
 #pragma unroll
@@ -387,8 +394,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
           v[e] = d.x;
           v[e + 1] = d.y;
         }
-        __stcs(out + i, Vec<T>::pack(v));
-      });
+        __stcs(o + b * threads, Vec<T>::pack(v));
+      }, [&] { o += kStep; });
       // single values, and the target's place once more by the thread that wrote it
       const float hit_share = g * (1.0f - r.smoothing);
       if (now.single >= 0) dx[now.single] = T::put(of(both(now.x_single)).x - (now.single == now.t ? hit_share : 0.0f));
