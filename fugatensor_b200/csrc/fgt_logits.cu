@@ -38,21 +38,29 @@ struct Listed {
 };
 
 // For a token that occurred or has a bias. x / repetition is x times the rounded
-// reciprocal (within 1.5 units of f32), and the count's share is one FMA.
+// reciprocal (within 1.5 units of f32); the count's share, with the presence
+// penalty, is one FMA, and a token that only has a bias is x * 1 - 0.
 struct Penalty {
   float repetition, inverse, presence, frequency;
   __device__ __forceinline__ Penalty(float r, float p, float f)
       : repetition(r), inverse(1.0f / r), presence(p), frequency(f) {}
   __device__ __forceinline__ float operator()(float x, unsigned count) const {
     const unsigned made = count & ~(kPrompt | kBiased | kTwice);
-    const float less = __fmul_rn(x, x > 0.0f ? inverse : repetition);
-    x = count & ~(kBiased | kTwice) ? less : x;
-    const float lower = __fsub_rn(__fmaf_rn(-frequency, (float)made, x), presence);
-    return made ? lower : x;
+    const bool occurred = count & ~(kBiased | kTwice);
+    const float factor = x > 0.0f ? inverse : repetition, less = __fmaf_rn(frequency, (float)made, presence);
+    return __fsub_rn(__fmul_rn(x, occurred ? factor : 1.0f), made ? less : 0.0f);
   }
 };
 
-template <class T>
+// One instruction where a token is outside the slice: d is its distance from the slice's first.
+FGT_DEV void count_token(unsigned counter, unsigned d, unsigned span) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.lt.u32 p, %1, %2;\n\t@p red.shared.add.u32 [%0], 1;\n\t}" ::"r"(counter + d * 4), "r"(d), "r"(span) : "memory");
+}
+FGT_DEV void mark_token(unsigned counter, unsigned d, unsigned span) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.lt.u32 p, %1, %2;\n\t@p red.shared.or.b32 [%0], %3;\n\t}" ::"r"(counter + d * 4), "r"(d), "r"(span), "r"(kPrompt) : "memory");
+}
+
+template <class T, bool kWide>  // kWide: the tokens are 64-bit
 __global__ void __launch_bounds__(kThreads, 3)
     adjust_slices(const typename T::S* __restrict__ logits, Rules r, int slices, int slice_vecs, typename T::S* __restrict__ out) {
   using E = typename T::S;
@@ -89,7 +97,7 @@ __global__ void __launch_bounds__(kThreads, 3)
   fetch(first + threadIdx.x);  // on its way while the history is counted
 
   // The row's history: `before` single tokens, then 16-byte vectors of `per` tokens, then single tokens.
-  const int per = r.tokens.wide ? 2 : 4, size = 16 / per;
+  constexpr int per = kWide ? 2 : 4, size = 16 / per;
   const char* const history = static_cast<const char*>(r.tokens.p) + row * r.history * size;
   const int before = min((int)((16 - ((uintptr_t)history & 15)) & 15) / size, (int)r.history);
   uint4 h[kHistoryBatch];
@@ -151,17 +159,13 @@ __global__ void __launch_bounds__(kThreads, 3)
   }
   if (n > 0) {
     const unsigned span = (unsigned)(high - low);
-    unsigned* const counter = count + (low - base + kLead);
-    auto prompted = [&](int t) {
-      if ((unsigned)(t - low) < span) atomicOr(counter + (t - low), kPrompt);
-    };
-    auto generated = [&](int t) {
-      if ((unsigned)(t - low) < span) atomicAdd(counter + (t - low), 1u);
-    };
+    const unsigned counter = (unsigned)__cvta_generic_to_shared(count + (low - base + kLead));
+    auto prompted = [&](int t) { mark_token(counter, (unsigned)(t - low), span); };
+    auto generated = [&](int t) { count_token(counter, (unsigned)(t - low), span); };
     auto visit = [&](int t, int i) { i < prompt ? prompted(t) : generated(t); };
     auto narrow = [](fgt_i64 t) { return t >> 31 ? -1 : (int)t; };  // -1: none that a vocabulary has
     auto single = [&](int i) {
-      visit(r.tokens.wide ? narrow(reinterpret_cast<const fgt_i64*>(history)[i]) : reinterpret_cast<const int*>(history)[i], i);
+      visit(kWide ? narrow(reinterpret_cast<const fgt_i64*>(history)[i]) : reinterpret_cast<const int*>(history)[i], i);
     };
     const int vectors = n > before ? (n - before) / per : 0, after = before + vectors * per;
     if (threadIdx.x < min(before, n)) single(threadIdx.x);
@@ -172,7 +176,7 @@ __global__ void __launch_bounds__(kThreads, 3)
       for (int b = 0; b < kHistoryBatch; ++b) {
         if (i0 + b * kThreads >= vectors) break;
         const int i = before + (i0 + b * kThreads) * per;
-        if (r.tokens.wide) {
+        if (kWide) {
           visit(narrow((fgt_i64)h[b].x | (fgt_i64)(int)h[b].y << 32), i);
           visit(narrow((fgt_i64)h[b].z | (fgt_i64)(int)h[b].w << 32), i + 1);
         } else if (i >= prompt) {
@@ -355,8 +359,9 @@ extern "C" fgt_status fgt_adjust_logits(const fgt_adjust_logits_desc* d, const f
       const bool listed = b->bias && d->biases <= kListed;
       const size_t smem = (b->tokens || listed ? (size_t)(kLead + slice_vecs * N + N + 3) / 4 * 16 : 0) +
                           (listed ? (size_t)d->biases * sizeof(Listed) : 0);
-      active_clusters(adjust_slices<T>, kThreads, smem, 1);  // leave for the shared memory
-      launch(Launch{(cudaStream_t)stream, programmatic((cudaStream_t)stream)}, adjust_slices<T>,
+      auto kernel = b->tokens && d->token_dtype == FGT_I64 ? adjust_slices<T, true> : adjust_slices<T, false>;
+      active_clusters(kernel, kThreads, smem, 1);  // leave for the shared memory
+      launch(Launch{(cudaStream_t)stream, programmatic((cudaStream_t)stream)}, kernel,
              blocks_for(size_product(d->rows, slices, "rows x vocab"), 1, "rows x vocab"), kThreads, smem, 1, (const E*)b->logits,
              r, slices, (int)slice_vecs, (E*)b->out);
     });
