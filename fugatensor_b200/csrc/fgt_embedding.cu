@@ -27,7 +27,7 @@ constexpr int kLookupThreads = 256, kLookupVecs = 4;
 template <class T, bool kVec>
 __global__ void __launch_bounds__(kLookupThreads)
     embedding_rows(const typename T::S* __restrict__ table, Index indices, fgt_i64 count, fgt_i64 vocab, fgt_i64 dim,
-                   float scale, typename T::S* __restrict__ out) {
+                   float scale, unsigned step_rows, unsigned step_vecs, typename T::S* __restrict__ out) {
   constexpr int N = Vec<T>::kN;
   grid_wait();
   grid_release();
@@ -35,15 +35,24 @@ __global__ void __launch_bounds__(kLookupThreads)
   const fgt_i64 first = blockIdx.x * (fgt_i64)(kLookupThreads * kLookupVecs) + threadIdx.x;
   uint4 v[kLookupVecs];
   if constexpr (kVec) {
-    const fgt_i64 per_row = dim / N;
+    // the first vector's row and place by a division, the others' by adding what kLookupThreads vectors are
+    const unsigned per_row = (unsigned)(dim / N);
+    fgt_i64 row = total >> 32 ? first / per_row : (fgt_i64)((unsigned)first / per_row);
+    unsigned col = (unsigned)(first - row * per_row);
+    const uint4* const rows = reinterpret_cast<const uint4*>(table);
 #pragma unroll
     for (int k = 0; k < kLookupVecs; ++k) {
-      const fgt_i64 at = first + k * kLookupThreads;
       v[k] = make_uint4(0, 0, 0, 0);
-      if (at * N >= total) continue;
-      const fgt_i64 row = total >> 32 ? at / per_row : (fgt_i64)((unsigned)at / (unsigned)per_row);
-      const fgt_i64 t = indices[row];
-      if (t >= 0 && t < vocab) v[k] = *reinterpret_cast<const uint4*>(table + t * dim + (at - row * per_row) * N);
+      if (row < count) {
+        const fgt_i64 t = indices[row];
+        if (t >= 0 && t < vocab) v[k] = rows[t * per_row + col];
+      }
+      row += step_rows;
+      col += step_vecs;
+      if (col >= per_row) {
+        col -= per_row;
+        ++row;
+      }
     }
 #pragma unroll
     for (int k = 0; k < kLookupVecs; ++k) {
@@ -692,6 +701,7 @@ void check(const fgt_embedding_desc* d) {
   require(is_float(d->dtype), "dtype must be f32, f16 or bf16");
   size_product(size_product(d->vocab, d->dim, "the table"), 4, "the table");
   size_product(size_product(d->count, d->dim, "indices x dim"), 4, "indices x dim");
+  require(d->dim < (INT64_C(1) << 31), "dim must be below 2^31");
 }
 
 // How the workspace of the gradient is laid out (bytes from its start).
@@ -757,7 +767,9 @@ extern "C" fgt_status fgt_embedding(const fgt_embedding_desc* d, const void* tab
       using T = decltype(t);
       using S = typename T::S;
       auto kernel = d->dim % n == 0 ? embedding_rows<T, true> : embedding_rows<T, false>;
-      launch(l, kernel, grid, kLookupThreads, 0, 1, (const S*)table, ids, d->count, d->vocab, d->dim, d->scale, (S*)out);
+      const unsigned per_row = (unsigned)std::max<int64_t>(1, d->dim / n);
+      launch(l, kernel, grid, kLookupThreads, 0, 1, (const S*)table, ids, d->count, d->vocab, d->dim, d->scale,
+             kLookupThreads / per_row, kLookupThreads % per_row, (S*)out);
     });
   });
 }
