@@ -8,6 +8,10 @@
 // history, and then streams its logits past the counters. A vector none of
 // whose tokens occurred is copied as it is. The few tokens with a bias are done
 // after the others, one thread each.
+// On B200 64 rows of 128000 bf16 with up to 4096 tokens, 32 biases and a mask
+// take 18 us (a copy of them 9: the rest is a chain of loads and barriers), 384
+// rows of 50021 f32 with up to 32768 tokens and 300 biases 57 us (a copy 24: the
+// rest is instructions, half of them for the history, which every slice reads).
 #include <type_traits>
 
 #include "fgt_vocab.cuh"

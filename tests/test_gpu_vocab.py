@@ -79,7 +79,7 @@ def test_embedding_grad(dtype, kind, n, vocab, dim):
         assert torch.equal(got.torch(), again.torch())  # no order of atomics in it
 
 
-@pytest.mark.parametrize("n,vocab,dim", [(40000, 300, 72), (70000, 131071, 16), (200000, 1000, 9), (131072, 300000, 4)])
+@pytest.mark.parametrize("n,vocab,dim", [(40000, 300, 72), (70000, 131071, 16), (200000, 1000, 9), (131072, 300000, 4), (300000, 5000, 12)])
 def test_embedding_grad_of_long_batches(n, vocab, dim):
     g = gen(3)
     ids = ids_like("text", n, vocab, g, "i32")
@@ -151,6 +151,47 @@ def test_cross_entropy(dtype, reduction, rows, vocab, eps, z):
     alone, grad_alone = make()[0], make()[1]
     R.check(alone.torch(), loss, lbound + R.U32 * loss.abs(), "loss alone")
     R.check(grad_alone.torch(), grad, R.rounded(gbound, grad, dtype), "gradient alone")
+
+
+@pytest.mark.parametrize("rows,vocab,dtype", [(20000, 1000, "bf16"), (9000, 257, "f32"), (3000, 8191, "f16"), (1200, 33000, "bf16"),
+                                              (300, 70000, "f16"), (80, 128000, "f32"), (30, 400003, "f32"), (70000, 5, "f32")])
+@pytest.mark.parametrize("eps", [0.0, 0.1])
+def test_cross_entropy_of_many_rows(rows, vocab, dtype, eps):
+    """Rows enough to fill the GPU: a warp, a CTA of every size, or a cluster walks several of them."""
+    g = gen(15)
+    x, t = loss_case(rows, vocab, dtype, "i32", g)
+    t[::7] = -100
+    seed = torch.tensor(2.0 ** 12, device="cuda")  # f16 gradients of a mean would underflow
+    loss, lbound, grad, gbound = R.cross_entropy(x, t, -100, eps, 0.0, "mean", seed)
+    X = R.wrap(x)
+    l = F.cross_entropy(X, R.wrap(t), label_smoothing=eps)
+    d = ft.grad(l, X, seed=R.wrap(seed))
+    ft.evaluate(l, d)
+    R.check(l.torch(), loss, lbound + R.U32 * loss.abs(), "loss")
+    R.check(d.torch(), grad, R.rounded(gbound, grad, dtype), "gradient")
+    again = F.cross_entropy(X, R.wrap(t), label_smoothing=eps)
+    assert torch.equal(again.torch(), l.torch())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_cross_entropy_of_rows_that_exceed_their_first_values(dtype):
+    """A thread takes its reference from its first values: here far larger ones follow, the sum
+    overflows, and the row is summed again; very large and very small rows likewise."""
+    g = gen(16)
+    x, t = loss_case(12, 5003, dtype, "i32", g)
+    x[0, 4000:] += 300.0
+    x[3, 2000] = 1e6
+    x[4] *= 1e30
+    x[5] -= 1e5
+    x[7, :4990] = -math.inf
+    t[7] = 5000
+    loss, lbound, grad, gbound = R.cross_entropy(x, t, reduction="none")
+    X = R.wrap(x)
+    l = F.cross_entropy(X, R.wrap(t), reduction="none")
+    d = ft.grad(l, X, seed=R.wrap(torch.ones(12, device="cuda")))
+    ft.evaluate(l, d)
+    R.check(l.torch(), loss, lbound + R.U32 * loss.abs())
+    R.check(d.torch(), grad, R.rounded(gbound, grad, dtype))
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -293,6 +334,21 @@ def test_adjust_logits_of_one_vector_and_of_a_batch_of_batches():
             assert torch.equal(one.torch(), out[i, j])
     none = F.adjust_logits(R.wrap(x), repetition=1.5, presence=0.25).torch()
     assert torch.equal(none, x)
+
+
+def test_tokens_beyond_32_bits_are_skipped():
+    x = torch.ones(1, 40, device="cuda")
+    far = torch.tensor([[3, 2 ** 32 + 5, 2 ** 40, -2 ** 40, -2 ** 63, 2 ** 31 + 7, 39]], device="cuda")
+    out = F.adjust_logits(R.wrap(x), R.wrap(far), presence=1.0, bias_tokens=R.wrap(far), bias=R.wrap(torch.full((1, 7), 0.5, device="cuda"))).torch()
+    want = torch.ones(1, 40, device="cuda")
+    want[0, 3] = want[0, 39] = 0.5
+    assert torch.equal(out, want)
+    table = torch.randn(40, 8, device="cuda")
+    y = F.embedding(R.wrap(table), R.wrap(far[0])).torch()
+    assert torch.equal(y[0], table[3]) and torch.equal(y[6], table[39]) and not y[1:6].any()
+    T = R.wrap(table)
+    d = ft.grad(F.embedding(T, R.wrap(far[0])), T, seed=R.wrap(torch.ones(7, 8, device="cuda"))).torch()
+    assert d[3].eq(1).all() and d[39].eq(1).all() and float(d.sum()) == 16.0
 
 
 def test_biases_of_one_token_add_in_their_order():
