@@ -24,19 +24,13 @@ import threading
 
 from . import dtypes as _dt
 from . import ir
-from .operators import NAMES as _OPERATORS
+from . import operators
 from .tensor import Tensor
-
-def _raw_stream(index):
-    """The current stream of CUDA device ``index`` as a raw handle."""
-    import torch
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # without building a Stream object
-    return torch.cuda.current_stream(index).cuda_stream if raw is None else raw(index)
-
 
 _ENGINES = {}
 _DEFAULT = ["cuda:0"]
 _LOCK = threading.RLock()
+_cuda = _raw_stream = None  # torch.cuda, and a device's current stream as a raw handle: set with the first device
 
 
 def _normalize_device(device):
@@ -240,75 +234,79 @@ class Engine:
         """Evaluate roots whose graph contains operators (operators.py): launches in dependency
         order, each after the partitions that compute what it reads, then the remaining roots as one
         partition. Values of tensors other than the roots live for this call only: they stay pending."""
-        import torch
-        from . import operators
         device = self._cuda_device()
-        index, known, ran, kept = device.index, {}, [], []
+        if _cuda.current_device() != device.index:
+            with _cuda.device(device):
+                return self._evaluate_operators(roots)
+        stream = _raw_stream(device.index)
         self.last_execution_plan = self.last_report = None
+        groups = operators.direct(roots)
+        if groups is None:
+            ran = self._run_graph(roots, device, stream)
+        else:
+            ran = []
+            for members in groups:
+                for t, o in zip(members, operators.launch(members, self._operand, stream)):
+                    ran.append(t._expr[0])
+                    t._data, t._expr, t._ops = o, None, False
+            self.stats["program_submissions"] += len(groups)
+        # of the last partition, if one ran; operators' kernels are not in it nor in stats["launches"]
+        self.last_report = {**self.last_report, "operators": ran} if self.last_report else {"operators": ran}
+
+    def _operand(self, t, known=None):
+        """A materialised tensor's buffer as an operator takes it: on this device, dense, 16-byte aligned."""
+        x = t._data if known is None else known
+        if x.get_device() != self._torch_device.index:
+            x = x.to(self._torch_device)
+        if not x.is_contiguous():
+            raise ValueError(f"operand must be a contiguous CUDA tensor, got {x.dtype}{list(x.shape)} with strides {x.stride()}")
+        return x.clone() if x.data_ptr() & 15 else x  # a slice (ids[1:]) may start anywhere
+
+    def _run_graph(self, roots, device, stream):
+        """The launches under ``roots`` in dependency order, with the partitions between them."""
+        known, ran = {}, []
 
         def data(t):
-            x = known[id(t)] if t._expr is not None else t._data
-            if x.get_device() != index:
-                x = x.to(device)
-            if not x.is_contiguous():
-                raise ValueError(f"operand must be a contiguous CUDA tensor, got {x.dtype}{list(x.shape)} with strides {x.stride()}")
-            if x.data_ptr() % 16:  # a slice (ids[1:]): the entry points take 16-byte aligned buffers
-                x = x.clone()
-                kept.append(x)
-            return x
+            return self._operand(t, known[id(t)] if t._expr is not None else None)
 
         def partition(wanted):
             desc, leaves, outs = self._trace(wanted, known)
             for t, o in zip(outs, self._run_partition(desc, leaves, known, device)):
                 known[id(t)] = o
 
-        def run(members, stream):
-            for t, o in zip(members, operators.launch(members, data, stream)):
-                known[id(t)] = o
-                ran.append(t._expr[0])
-            self.stats["program_submissions"] += 1
-
-        def run_all():
-            stream = _raw_stream(index)
-            groups = operators.direct(roots)
-            if groups is not None:
-                for members in groups:
-                    run(members, stream)
-                return
-            todo = operators.units(roots)
-            done = set()
-            while len(done) < len(todo):
-                ready = [i for i, (_, needs) in enumerate(todo) if i not in done and needs <= done]
-                wanted = {id(a): a for i in ready for t in todo[i][0] for a in t._expr[1]
-                          if a._expr is not None and id(a) not in known}
-                if wanted:
-                    partition(list(wanted.values()))
-                for i in ready:
-                    run(todo[i][0], stream)
-                done.update(ready)
-            rest = [r for r in roots if id(r) not in known]
-            if rest:
-                partition(rest)
-
-        if torch.cuda.current_device() == index:
-            run_all()
-        else:
-            with torch.cuda.device(device):
-                run_all()
-        # of the last partition, if one ran; operators' kernels are not in it nor in stats["launches"]
-        self.last_report = {**(self.last_report or {}), "operators": ran}
+        todo = operators.units(roots)
+        done = set()
+        while len(done) < len(todo):
+            ready = [i for i, (_, needs) in enumerate(todo) if i not in done and needs <= done]
+            wanted = {id(a): a for i in ready for t in todo[i][0] for a in t._expr[1]
+                      if a._expr is not None and id(a) not in known}
+            if wanted:
+                partition(list(wanted.values()))
+            for i in ready:
+                members = todo[i][0]
+                for t, o in zip(members, operators.launch(members, data, stream)):
+                    known[id(t)] = o
+                    ran.append(t._expr[0])
+            self.stats["program_submissions"] += len(ready)
+            done.update(ready)
+        rest = [r for r in roots if id(r) not in known]
+        if rest:
+            partition(rest)
         for r in roots:
-            r._data = known[id(r)]
-            r._expr = None
-            r._ops = False
+            r._data, r._expr, r._ops = known[id(r)], None, False
+        return ran
 
     def _cuda_device(self):
         """This engine's torch device; raises where there is none."""
-        import torch
         if self._torch_device is None:
+            global _cuda, _raw_stream
+            import torch
             from . import _fgt
             if not torch.cuda.is_available():
                 raise _fgt.CUDAError(4, "no CUDA device: fugatensor_b200 has no CPU execution path")
+            # without building a Stream object, where torch has that
+            _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda i: torch.cuda.current_stream(i).cuda_stream)
+            _cuda = torch.cuda
             self._torch_device = torch.device(self.device)
         return self._torch_device
 
@@ -380,7 +378,7 @@ def _hashable(attrs):
 
 
 def _build(g, op, argv, attrs):
-    if op in _OPERATORS:
+    if op in operators.NAMES:
         raise TypeError(f"{op} is an operator of its own, not part of a partition: use evaluate")
     if op == "constant":
         return g.constant(attrs[0], attrs[1])
