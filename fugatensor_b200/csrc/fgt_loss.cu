@@ -309,21 +309,23 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
       sum[0] = Exponent<true>(stat.c)(make_float2(now.x_single, kNegInf));
     }
     if (now.single >= 0) all.x = now.x_single;
+    Exponent<true> exp2(stat.c);
     each(end - first, [&](int b, const uint4& u) {
       float v[N];
       Vec<T>::unpack(u, v);
+      if (kAll)
+#pragma unroll
+        for (int e = 0; e < N; e += 2) all = __fadd2_rn(all, make_float2(v[e], v[e + 1]));
       if (stat.c == kNegInf) {
         float m = v[0];
 #pragma unroll
         for (int e = 1; e < N; ++e) m = fgt_fmax(m, v[e]);
-        if (m != kNegInf) stat.c = reference(m);
+        if (m == kNegInf) return;
+        stat.c = reference(m);
+        exp2 = Exponent<true>(stat.c);
       }
-      const Exponent<true> exp2(fmaxf(stat.c, -3e38f));
 #pragma unroll
-      for (int e = 0; e < N; e += 2) {
-        sum[b % 2] = __fadd2_rn(sum[b % 2], exp2(make_float2(v[e], v[e + 1])));
-        if (kAll) all = __fadd2_rn(all, make_float2(v[e], v[e + 1]));
-      }
+      for (int e = 0; e < N; e += 2) sum[b % 2] = __fadd2_rn(sum[b % 2], exp2(make_float2(v[e], v[e + 1])));
     }, [] {});
     for (;; whole = false) {
       const float2 both_sums = __fadd2_rn(sum[0], sum[1]);
