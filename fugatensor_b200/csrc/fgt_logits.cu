@@ -9,9 +9,12 @@
 // whose tokens occurred is copied as it is. The few tokens with a bias are done
 // after the others, one thread each.
 // On B200 64 rows of 128000 bf16 with up to 4096 tokens, 32 biases and a mask
-// take 18 us (a copy of them 9: the rest is a chain of loads and barriers), 384
-// rows of 50021 f32 with up to 32768 tokens and 300 biases 57 us (a copy 24: the
+// take 17 us (a copy of them 9: the rest is a chain of loads and barriers), 384
+// rows of 50021 f32 with up to 32768 tokens and 300 biases 55 us (a copy 24: the
 // rest is instructions, half of them for the history, which every slice reads).
+// Registers are what it is short of: three CTAs per SM leave 40 per thread, and
+// four vectors of history in flight in place of two spill (73 us); two CTAs of
+// larger slices read the history half as often but take 61 us.
 #include <type_traits>
 
 #include "fgt_vocab.cuh"
@@ -21,7 +24,7 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kBatch = 2;                  // vectors of logits per thread in flight, besides those at work
-constexpr int kHistoryBatch = 4;           // vectors of tokens per thread in flight
+constexpr int kHistoryBatch = 2;           // vectors of tokens per thread in flight
 constexpr int kLead = 8;                   // counters before a slice's first vector: a row's single values
 constexpr int kListed = kThreads;          // biases per row that a slice's list has room for
 constexpr unsigned kPrompt = 0x80000000u;  // a counter's top bits: the token is in the prompt,
@@ -87,30 +90,31 @@ __global__ void __launch_bounds__(kThreads, 3)
   const unsigned* const allowed = r.allowed ? r.allowed + row * r.words : nullptr;
   uint4 u[kBatch];
   unsigned bits[kBatch];  // of vector u: bit e set = its value e may be chosen
-  auto fetch = [&](int i0) {
-#pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const int i = i0 + b * kThreads;
-      if (i >= end) continue;
-      u[b] = __ldcs(in + i);
-      if (!allowed) continue;
-      const int t = lead + i * N;
-      bits[b] = __funnelshift_r(allowed[t >> 5], (t & 31) + N > 32 ? allowed[(t >> 5) + 1] : 0u, t & 31);
-    }
+  const uint4* src = in + (first + threadIdx.x);  // this thread's next vectors, kThreads apart,
+  int t0 = lead + (first + threadIdx.x) * N;      // and the first one's token
+  int left = end - first - threadIdx.x;           // one more vector for every kThreads of them
+  auto fetch = [&](int b, int ahead) {            // vector `ahead + b` from here into slot b, if there is one
+    if (left <= (ahead + b) * kThreads) return;
+    u[b] = __ldcs(src + (ahead + b) * kThreads);
+    if (!allowed) return;
+    const int t = t0 + (ahead + b) * (kThreads * N);
+    bits[b] = __funnelshift_r(allowed[t >> 5], (t & 31) + N > 32 ? allowed[(t >> 5) + 1] : 0u, t & 31);
   };
-  fetch(first + threadIdx.x);  // on its way while the history is counted
+#pragma unroll
+  for (int b = 0; b < kBatch; ++b) fetch(b, 0);  // on their way while the history is counted
 
   // The row's history: `before` single tokens, then 16-byte vectors of `per` tokens, then single tokens.
   constexpr int per = kWide ? 2 : 4, size = 16 / per;
   const char* const history = static_cast<const char*>(r.tokens.p) + row * r.history * size;
   const int before = min((int)((16 - ((uintptr_t)history & 15)) & 15) / size, (int)r.history);
   uint4 h[kHistoryBatch];
-  auto recall = [&](int i0, int vectors) {
+  const uint4* past = reinterpret_cast<const uint4*>(history + before * size) + threadIdx.x;
+  if (r.tokens.p) {  // before the lengths are known
+    const int vectors = ((int)r.history - before) / per;
 #pragma unroll
     for (int b = 0; b < kHistoryBatch; ++b)
-      if (i0 + b * kThreads < vectors) h[b] = __ldcs(reinterpret_cast<const uint4*>(history + before * size) + i0 + b * kThreads);
-  };
-  if (r.tokens.p) recall(threadIdx.x, ((int)r.history - before) / per);  // before the lengths are known
+      if ((int)threadIdx.x + b * kThreads < vectors) h[b] = __ldcs(past + b * kThreads);
+  }
 
   // The slice's biases in their order: each warp appends its own after those of the warps before.
   const int counters = (kLead + slice_vecs * N + N + 3) / 4 * 4;
@@ -174,25 +178,34 @@ __global__ void __launch_bounds__(kThreads, 3)
     const int vectors = n > before ? (n - before) / per : 0, after = before + vectors * per;
     if (threadIdx.x < min(before, n)) single(threadIdx.x);
     if (after + threadIdx.x < n) single(after + threadIdx.x);  // fewer than `per`
-    for (int i0 = threadIdx.x; i0 < vectors; i0 += kHistoryBatch * kThreads) {
-      if (i0 != threadIdx.x) recall(i0, vectors);
+    int given = prompt - before - (int)threadIdx.x * per;  // tokens of the prompt from this thread's next vector on
+    constexpr int step = kHistoryBatch * kThreads;
+    for (int ahead = vectors - (int)threadIdx.x; ahead > 0; ahead -= step, given -= step * per, past += step) {
 #pragma unroll
       for (int b = 0; b < kHistoryBatch; ++b) {
-        if (i0 + b * kThreads >= vectors) break;
-        const int i = before + (i0 + b * kThreads) * per;
+        if (ahead <= b * kThreads) break;
+        const uint4 t = h[b];
+        if (ahead > step + b * kThreads) h[b] = __ldcs(past + step + b * kThreads);
+        const int g = given - b * (kThreads * per);
         if (kWide) {
-          visit(narrow((fgt_i64)h[b].x | (fgt_i64)(int)h[b].y << 32), i);
-          visit(narrow((fgt_i64)h[b].z | (fgt_i64)(int)h[b].w << 32), i + 1);
-        } else if (i >= prompt) {
-          generated((int)h[b].x);
-          generated((int)h[b].y);
-          generated((int)h[b].z);
-          generated((int)h[b].w);
-        } else {
-          visit((int)h[b].x, i);
-          visit((int)h[b].y, i + 1);
-          visit((int)h[b].z, i + 2);
-          visit((int)h[b].w, i + 3);
+          const int t0 = narrow((fgt_i64)t.x | (fgt_i64)(int)t.y << 32), t1 = narrow((fgt_i64)t.z | (fgt_i64)(int)t.w << 32);
+          g > 0 ? prompted(t0) : generated(t0);
+          g > 1 ? prompted(t1) : generated(t1);
+        } else if (g <= 0) {
+          generated((int)t.x);
+          generated((int)t.y);
+          generated((int)t.z);
+          generated((int)t.w);
+        } else if (g >= per) {
+          prompted((int)t.x);
+          prompted((int)t.y);
+          prompted((int)t.z);
+          prompted((int)t.w);
+        } else {  // the prompt ends in this vector
+          prompted((int)t.x);
+          g > 1 ? prompted((int)t.y) : generated((int)t.y);
+          g > 2 ? prompted((int)t.z) : generated((int)t.z);
+          generated((int)t.w);
         }
       }
     }
@@ -220,21 +233,18 @@ __global__ void __launch_bounds__(kThreads, 3)
   }
 
   constexpr unsigned kMinusInf = sizeof(E) == 4 ? 0xff800000u : std::is_same<T, F16>::value ? 0xfc00u : 0xff80u;
-  for (int i0 = first + threadIdx.x; i0 < end; i0 += kBatch * kThreads) {
-    uint4 now[kBatch];
-    unsigned may[kBatch];
+  constexpr int step = kBatch * kThreads;
+  uint4* to = reinterpret_cast<uint4*>(y + lead) + (first + threadIdx.x);
+  const uint4* counts = reinterpret_cast<const uint4*>(count + kLead) + threadIdx.x * (N / 4);
+  for (; left > 0; left -= step, src += step, to += step, counts += step * (N / 4), t0 += step * N) {
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
-      now[b] = u[b];
-      may[b] = bits[b];
-    }
-    fetch(i0 + kBatch * kThreads);
-#pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const int i = i0 + b * kThreads;
-      if (i >= end) break;
+      if (left <= b * kThreads) break;
+      uint4 now = u[b];
+      const unsigned may = bits[b];
+      fetch(b, kBatch);
       if (r.tokens.p) {
-        const uint4* c = reinterpret_cast<const uint4*>(count + kLead) + (i - first) * (N / 4);
+        const uint4* c = counts + b * (kThreads * (N / 4));
         uint4 n[N / 4];
         unsigned some = 0;
 #pragma unroll
@@ -244,33 +254,35 @@ __global__ void __launch_bounds__(kThreads, 3)
         }
         if (some) {
           float v[N];
-          Vec<T>::unpack(now[b], v);
+          Vec<T>::unpack(now, v);
 #pragma unroll
           for (int k = 0; k < N / 4; ++k) {
-            // (a branch that no lane takes is worth a vote)
+            // of 8 tokens a vector many occurred in no lane's (a vote); of 4, in a long history, few: 55.3 us
+            // against 56.6 with votes for 384 x 50021 f32
             const unsigned lanes = __activemask();
-            if (__any_sync(lanes, n[k].x)) v[4 * k] = penalty(v[4 * k], n[k].x);
-            if (__any_sync(lanes, n[k].y)) v[4 * k + 1] = penalty(v[4 * k + 1], n[k].y);
-            if (__any_sync(lanes, n[k].z)) v[4 * k + 2] = penalty(v[4 * k + 2], n[k].z);
-            if (__any_sync(lanes, n[k].w)) v[4 * k + 3] = penalty(v[4 * k + 3], n[k].w);
+            auto any = [&](unsigned c) { return N == 4 || __any_sync(lanes, c); };
+            if (any(n[k].x)) v[4 * k] = penalty(v[4 * k], n[k].x);
+            if (any(n[k].y)) v[4 * k + 1] = penalty(v[4 * k + 1], n[k].y);
+            if (any(n[k].z)) v[4 * k + 2] = penalty(v[4 * k + 2], n[k].z);
+            if (any(n[k].w)) v[4 * k + 3] = penalty(v[4 * k + 3], n[k].w);
           }
-          now[b] = Vec<T>::pack(v);
+          now = Vec<T>::pack(v);
         }
       }
       if (allowed) {
-        unsigned w[4] = {now[b].x, now[b].y, now[b].z, now[b].w};
+        unsigned w[4] = {now.x, now.y, now.z, now.w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           if (sizeof(E) == 4) {
-            w[k] = may[b] >> k & 1 ? w[k] : kMinusInf;
+            w[k] = may >> k & 1 ? w[k] : kMinusInf;
           } else {
-            const unsigned keep = (may[b] >> (2 * k) & 1 ? 0xffffu : 0) | (may[b] >> (2 * k + 1) & 1 ? 0xffff0000u : 0);
+            const unsigned keep = (may >> (2 * k) & 1 ? 0xffffu : 0) | (may >> (2 * k + 1) & 1 ? 0xffff0000u : 0);
             w[k] = (w[k] & keep) | (kMinusInf * 0x10001u & ~keep);
           }
         }
-        now[b] = make_uint4(w[0], w[1], w[2], w[3]);
+        now = make_uint4(w[0], w[1], w[2], w[3]);
       }
-      __stcs(reinterpret_cast<uint4*>(y + lead) + i, now[b]);
+      __stcs(to + b * kThreads, now);
     }
   }
 
