@@ -279,6 +279,12 @@ def grad(outputs, inputs, *, seed=None):
     Tensor, a tuple/list returns a tuple.
     """
     single_out = isinstance(outputs, Tensor)
+    if single_out and outputs._ops and isinstance(inputs, Tensor) and inputs._expr is None and (
+            outputs._shape == () if seed is None else
+            isinstance(seed, Tensor) and seed._shape == outputs._shape and seed._dtype is outputs._dtype):
+        got = operators.vjp_direct(outputs, inputs, seed)
+        if got is not None:
+            return got
     outs = [outputs] if single_out else list(outputs)
     single_in = isinstance(inputs, Tensor)
     ins = [inputs] if single_in else list(inputs)
@@ -305,10 +311,6 @@ def grad(outputs, inputs, *, seed=None):
             raise ValueError("seed must match its output's shape and dtype")
         resolved.append(s)
 
-    if single_out and single_in and ins[0]._expr is None and outs[0]._ops:
-        got = operators.vjp_direct(outs[0], ins[0], resolved[0])
-        if got is not None:
-            return got
     order = _topo(outs)
     in_ids = {id(t) for t in ins}
     # activity: depends (differentiably) on a requested input

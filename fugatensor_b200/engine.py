@@ -254,13 +254,18 @@ class Engine:
         self.last_report = {**self.last_report, "operators": ran} if self.last_report else {"operators": ran}
 
     def _operand(self, t, known=None):
-        """A materialised tensor's buffer as an operator takes it: on this device, dense, 16-byte aligned."""
+        """A materialised tensor's buffer as an operator takes it (on this device, dense, 16-byte
+        aligned), and its address."""
         x = t._data if known is None else known
         if x.get_device() != self._torch_device.index:
             x = x.to(self._torch_device)
         if not x.is_contiguous():
             raise ValueError(f"operand must be a contiguous CUDA tensor, got {x.dtype}{list(x.shape)} with strides {x.stride()}")
-        return x.clone() if x.data_ptr() & 15 else x  # a slice (ids[1:]) may start anywhere
+        p = x.data_ptr()
+        if p & 15:  # a slice (ids[1:]) may start anywhere
+            x = x.clone()
+            p = x.data_ptr()
+        return x, p
 
     def _run_graph(self, roots, device, stream):
         """The launches under ``roots`` in dependency order, with the partitions between them."""

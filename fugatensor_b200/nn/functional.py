@@ -197,20 +197,18 @@ def adjust_logits(logits, tokens=None, lengths=None, *, prompt_lengths=None, rep
     batch, vocab = logits._shape[:-1], logits._shape[-1]
     names, args = ["logits"], [logits]
 
-    def take(name, x, kinds, shape):
+    def take(name, x, kinds, shape=None):  # None: the batch's, with a length of its own
         _tensor(x, name, kinds, logits)
+        if shape is None:
+            shape = batch + x._shape[-1:]
         if x._shape != shape:
             raise ValueError(f"{name} must have shape {shape}, got {x._shape}")
         if 0 not in shape:  # nothing in it: as if it had not been given
             names.append(name)
             args.append(x)
 
-    def columns(name, x, kinds):
-        _tensor(x, name, kinds, logits)
-        take(name, x, kinds, batch + x._shape[-1:])
-
     if tokens is not None:
-        columns("tokens", tokens, _INDEX)
+        take("tokens", tokens, _INDEX)
         for name, x in (("lengths", lengths), ("prompt_lengths", prompt_lengths)):
             if x is not None:
                 take(name, x, _INDEX, batch)
@@ -232,7 +230,7 @@ def adjust_logits(logits, tokens=None, lengths=None, *, prompt_lengths=None, rep
     if (bias is None) != (bias_tokens is None):
         raise ValueError("bias and bias_tokens are given together")
     if bias is not None:
-        columns("bias_tokens", bias_tokens, _INDEX)
+        take("bias_tokens", bias_tokens, _INDEX)
         take("bias", bias, ("f32",), bias_tokens._shape)
     if allowed is not None:
         take("allowed", allowed, ("i32",), batch + (-(-vocab // 32),))

@@ -52,7 +52,7 @@ def _scalar(t, depth=4):
 
 # ------------------------------------------------------------- gradients ---
 def vjp(t, g, active):
-    """Cotangents of an operator's operands given its cotangent ``g``."""
+    """Cotangents of an operator's operands given its cotangent ``g`` (None: the number one)."""
     op, args, attrs = t._expr
     if op == "embedding":
         table, indices = args
@@ -61,7 +61,7 @@ def vjp(t, g, active):
         return [grad if active[0] else None, None]
     if op == "cross_entropy":
         logits, targets = args
-        value = _scalar(g)
+        value = 1.0 if g is None else _scalar(g)
         seed, scale = ((), value) if value is not None else ((g,), 1.0)
         return [node("cross_entropy_grad", (logits, targets) + seed, attrs + (scale,), logits._dtype, logits._shape), None]
     from .autograd import DifferentiationError
@@ -195,7 +195,8 @@ def direct(roots):
 
 # -------------------------------------------------------------- launches ---
 def launch(members, data, stream):
-    """Run one launch on raw ``stream``; ``data(tensor)`` gives an operand's buffer. Returns the members' results."""
+    """Run one launch on raw ``stream``; ``data(tensor)`` gives an operand's buffer, which is kept until
+    the launch is enqueued, and its address. Returns the members' results."""
     if _native is None:
         _load()
     return _LAUNCH[members[-1]._expr[0]](members, data, stream)
@@ -224,24 +225,23 @@ def _check(status):
 def _embedding(members, data, stream):
     (t,) = members
     (table, indices), (scale, padding) = t._expr[1:]
-    tb, ib = data(table), data(indices)
+    (tb, table_at), (ib, ids_at) = data(table), data(indices)
     out = _empty(t, tb)
     _check(_native.embedding(_DT[t._dtype.ir], _DT[indices._dtype.ir], table._shape[0], table._shape[1], ib.numel(),
-                             scale, tb.data_ptr(), ib.data_ptr(), out.data_ptr(), stream))
+                             scale, table_at, ids_at, out.data_ptr(), stream))
     return (out,)
 
 
 def _embedding_grad(members, data, stream):
     (t,) = members
     (indices, g), (vocab, scale, padding) = t._expr[1:]
-    ib, gb = data(indices), data(g)
+    (ib, ids_at), (gb, g_at) = data(indices), data(g)
     out = _empty(t, gb)
     desc = (_DT[t._dtype.ir], _DT[indices._dtype.ir], vocab, t._shape[1], ib.numel(), scale,
             -1 if padding is None else padding)
     size = _native.embedding_grad_workspace(*desc)
     ws = _workspace(size, gb)
-    _check(_native.embedding_grad(*desc, ib.data_ptr(), gb.data_ptr(), out.data_ptr(), ws.data_ptr() if size else 0, size,
-                                  stream))
+    _check(_native.embedding_grad(*desc, ids_at, g_at, out.data_ptr(), ws.data_ptr() if size else 0, size, stream))
     return (out,)
 
 
@@ -255,41 +255,45 @@ def _cross_entropy(members, data, stream):
     args, attrs = (loss if grad is None else grad)._expr[1:]
     logits, targets = args[:2]
     ignore, smoothing, z, reduction = attrs[:4]
-    xb, tb = data(logits), data(targets)
-    seed = data(args[2]) if len(args) == 3 else None
+    (xb, logits_at), (tb, targets_at) = data(logits), data(targets)
+    seed, seed_at = data(args[2]) if len(args) == 3 else (None, 0)
     loss_out = None if loss is None else _empty(loss, xb)
     grad_out = None if grad is None else torch.empty_like(xb)
     desc = (_DT[logits._dtype.ir], _DT[targets._dtype.ir], REDUCTIONS[reduction], smoothing, z,
             1.0 if grad is None else attrs[4], tb.numel(), logits._shape[-1], ignore)
     size = _native.cross_entropy_workspace(*desc)
     ws = _workspace(size, xb)
-    _check(_native.cross_entropy(*desc, xb.data_ptr(), tb.data_ptr(), 0 if seed is None else seed.data_ptr(),
-                                 0 if loss is None else loss_out.data_ptr(), 0 if grad is None else grad_out.data_ptr(),
-                                 ws.data_ptr() if size else 0, size, stream))
+    _check(_native.cross_entropy(*desc, logits_at, targets_at, seed_at, 0 if loss is None else loss_out.data_ptr(),
+                                 0 if grad is None else grad_out.data_ptr(), ws.data_ptr() if size else 0, size, stream))
     return [loss_out if t is loss else grad_out for t in members]
+
+
+# the operands' places in the native call
+_RULES = {name: i for i, name in enumerate(("logits", "tokens", "lengths", "prompt_lengths", "repetition", "presence",
+                                            "frequency", "bias_tokens", "bias", "allowed"))}
 
 
 def _adjust_logits(members, data, stream):
     (t,) = members
     args, (names, repetition, presence, frequency) = t._expr[1:]
-    kept = {name: data(a) for name, a in zip(names, args)}  # alive until the launch
-    ptr = {name: b.data_ptr() for name, b in kept.items()}.get
-    given = dict(zip(names, args))
-
-    def last(name):  # an operand's last dimension, and its dtype
-        a = given.get(name)
-        return (0, 1) if a is None else (a._shape[-1] if a._shape else 0, _DT[a._dtype.ir])
-
-    x = kept["logits"]
+    at, kept = [0] * len(_RULES), []
+    token = length = bias_token = 1  # dtypes of what is not given: any
+    history = biases = 0
+    for name, a in zip(names, args):
+        i = _RULES[name]
+        buffer, at[i] = data(a)
+        kept.append(buffer)
+        if i == 1:
+            token, history = _DT[a._dtype.ir], a._shape[-1]
+        elif i in (2, 3):
+            length = _DT[a._dtype.ir]
+        elif i == 7:
+            bias_token, biases = _DT[a._dtype.ir], a._shape[-1]
+    x = kept[0]
     out = torch.empty_like(x)
     vocab = t._shape[-1]
-    (history, token), (biases, _), (_, bias_token) = last("tokens"), last("bias"), last("bias_tokens")
-    length = last("lengths" if "lengths" in given else "prompt_lengths")[1]
-    _check(_native.adjust_logits(
-        _DT[t._dtype.ir], token, length, bias_token, x.numel() // vocab if vocab else 0, vocab, history, biases, repetition,
-        presence, frequency, ptr("logits"), ptr("tokens", 0), ptr("lengths", 0), ptr("prompt_lengths", 0),
-        ptr("repetition", 0), ptr("presence", 0), ptr("frequency", 0), ptr("bias_tokens", 0), ptr("bias", 0),
-        ptr("allowed", 0), out.data_ptr(), stream))
+    _check(_native.adjust_logits(_DT[t._dtype.ir], token, length, bias_token, x.numel() // vocab if vocab else 0, vocab,
+                                 history, biases, repetition, presence, frequency, *at, out.data_ptr(), stream))
     return (out,)
 
 
