@@ -143,9 +143,9 @@ __global__ void __launch_bounds__(kCountThreads)
 // Bound by memory for f32 and long rows, by instructions (two exponentials a
 // value, and about 300 instructions per warp and row) for 16-bit and short
 // ones. On B200: 4096 x 32000 f32, loss alone, 82 us (0.98 of a copy's rate);
-// 2048 x 128000 f32 with the gradient 370 us (0.87); 8192 x 128000 bf16 696 us
-// (0.92), 760 to 810 where the power cap has lowered the clock; 8192 x 32000
-// bf16 188 us (0.85); 2048 x 50021 f16 95 us (0.66). Rows held in registers,
+// 2048 x 128000 f32 with the gradient 370 us (0.87); 8192 x 128000 bf16 677 us
+// (0.95), 740 to 790 where the power cap has lowered the clock; 8192 x 32000
+// bf16 188 us (0.85); 2048 x 50021 f16 93 us (0.67). Rows held in registers,
 // shared by a cluster, took 1250 us for the bf16 case (each phase waits for the
 // one before); a ring of whole row slices per cluster 1350 to 3400 us.
 enum Group { kWarp, kCta, kCluster };
