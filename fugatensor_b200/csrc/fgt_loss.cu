@@ -17,11 +17,14 @@ struct Row {
 
 // Exponentials are taken as 2^(x log2(e) - c) with c a whole number near the
 // largest x log2(e): the product and the difference are one FMA, and partial
-// sums with different c are brought together by exact powers of two. The row's
+// sums with different c are brought together by exact powers of two. A factor
+// below 2^-126 is flushed to 0, so a sum that has grown large gives its exponent
+// to c first (settle): what is lost is below 2^-80 of the row's sum. The row's
 // sum of exponentials is 2^c s, so lse = (c + log2(s)) ln 2. Rows that leave
 // f32's range that way (overflow where the first values do not show the
-// largest, values near the type's lowest, NaN) are computed as
-// 2^((x - m) log2(e)) with m the maximum.
+// largest, values near the type's lowest, NaN), and rows so far from zero that
+// not every whole number is an f32 value, are computed as 2^((x - m) log2(e))
+// with m the maximum.
 constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
 constexpr float kNegInf = -__builtin_huge_valf();
 
@@ -156,6 +159,23 @@ constexpr int kWarpGroups = 4;          // warps of a CTA that has a row per war
 struct Stat {
   float c, s, all;
 };
+
+// A large s gives its exponent to c. At a join the factor of a smaller c is 0
+// from 2^-127 on, and s must not be what would have made up for it: below 2^30,
+// and with 8192 threads at most to a row, all that is lost is 2^-83, while the
+// largest c's own s is 2^-0.5 or more. Settled once more, the row's s leaves g / s
+// a normal number. Where c + e is no f32 value s becomes infinite, which calls for
+// the second attempt; infinities and NaN stay.
+constexpr float kSettled = 1073741824.0f;  // 2^30
+constexpr float kWholes = 16777216.0f;     // 2^24: below, every whole number is an f32 value
+FGT_DEV void settle(Stat& a) {
+  if (!(a.s >= kSettled)) return;
+  const unsigned bits = __float_as_uint(a.s);
+  const float e = (float)((int)(bits >> 23) - 127), c = __fadd_rn(a.c, e);
+  const bool exact = __fsub_rn(c, a.c) == e && bits < 0x7f800000u;
+  a.s = __uint_as_float(exact ? (bits & 0x7fffffu) | 0x3f800000u : 0x7f800000u);
+  a.c = exact ? c : a.c;
+}
 
 // The statistics of a warp's lanes joined; every lane gets the result.
 template <bool kAll> __device__ __forceinline__ Stat warp_join(Stat a, bool whole) {
@@ -331,6 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
       const float2 both_sums = __fadd2_rn(sum[0], sum[1]);
       stat.s = both_sums.x + both_sums.y;
       stat.all = all.x + all.y;
+      if (whole) settle(stat);
       stat = warp_join<kAll>(stat, whole);
       if (G != kWarp) {
         Stat* slot = &s_stat[parity][cta * warps + warp];
@@ -358,7 +379,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
         stat = warp_join<kAll>(total, whole);
         parity ^= 1;  // the next exchange's writers do not meet this one's readers
       }
-      if (!whole || (stat.s > 0.0f && stat.s < __int_as_float(0x7f800000))) break;  // the same decision for the whole group
+      if (whole) settle(stat);  // the row's, for the gradient's factor
+      if (!whole || (stat.s > 0.0f && stat.s < __int_as_float(0x7f800000) && fabsf(stat.c) < kWholes)) break;  // the same decision for the whole group
       const uint4* in = reinterpret_cast<const uint4*>(logits + row * r.vocab + now.lead);
       float m = now.x_single;
       for (int i = first + me; i < end; i += threads) {

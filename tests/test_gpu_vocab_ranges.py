@@ -1,0 +1,103 @@
+"""Vocabulary operators at the ends of their ranges, against 64-bit references."""
+import pytest
+import torch
+
+import fugatensor_b200 as ft
+import fugatensor_b200.nn.functional as F
+from tests import _vocab as R
+
+pytestmark = pytest.mark.gpu
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+# --------------------------------------------- cross-entropy, wide rows ----
+# Exponentials below 2^-126 of a row's reference are 0 (ex2.approx.ftz), and the sum that they are
+# divided by is at least half a reference: a gradient is off by up to 2^-125 of its seed that way.
+FLUSHED = 2.0 ** -124
+
+
+def check_rows(x, t, dtype, eps=0.0):
+    """Row losses and gradients, together and the loss alone, with a seed per row."""
+    seed = 0.5 + torch.rand(x.shape[0], device="cuda", generator=gen(1))
+    # neither changes when a row is shifted; at its largest value the reference loses nothing to lse's size
+    shifted = x.double() - x.double().amax(1, keepdim=True)
+    loss, _, grad, gbound = R.cross_entropy(shifted, t, eps=eps, reduction="none", seed=seed)
+    lbound = R.cross_entropy(x, t, eps=eps, reduction="none")[1]
+    X, T = R.wrap(x), R.wrap(t)
+    l = F.cross_entropy(X, T, label_smoothing=eps, reduction="none")
+    d = ft.grad(l, X, seed=R.wrap(seed))
+    ft.evaluate(l, d)
+    R.check(l.torch(), loss, lbound + R.U32 * loss.abs(), "loss")
+    R.check(d.torch(), grad, R.rounded(gbound + FLUSHED * seed[:, None].double(), grad, dtype), "gradient")
+    alone = F.cross_entropy(X, T, label_smoothing=eps, reduction="none").torch()
+    R.check(alone, loss, lbound + R.U32 * loss.abs(), "loss alone")
+
+
+# a warp, a CTA, a cluster per row, and a CTA of 64 threads over many rows; `block` is what the group's
+# threads read first: every other block is low, so a thread's reference is far below its later values
+@pytest.mark.parametrize("dtype,rows,vocab,block", [
+    ("f32", 12, 500, 128), ("f32", 12, 5003, 2048), ("f32", 12, 32001, 2048), ("f32", 4200, 2400, 256),
+    ("f16", 12, 500, 256), ("f16", 12, 5003, 2048), ("f16", 12, 50021, 4096),
+    ("bf16", 12, 500, 256), ("bf16", 12, 5003, 2048), ("bf16", 12, 50021, 4096)])
+@pytest.mark.parametrize("eps", [0.0, 0.1])
+@pytest.mark.parametrize("rest", [-5.0, -9.0])
+def test_cross_entropy_of_rows_whose_first_values_are_far_below_the_others(dtype, rows, vocab, block, eps, rest):
+    g = gen(21)
+    depth = torch.tensor([80, 84, 86, 87, 88, 88.5, 89, 90, 91, 92, 95, 100], device="cuda")
+    x = torch.randn(rows, vocab, device="cuda", generator=g) * 0.5 + rest
+    low = (torch.arange(vocab, device="cuda") // block) % 2 == 0
+    x = torch.where(low[None, :], -depth[torch.arange(rows, device="cuda") % 12, None], x)
+    x[:, 0] = 0.0
+    t = torch.randint(0, vocab, (rows,), device="cuda", generator=g)
+    check_rows(x.to(R.TORCH[dtype]), t, dtype, eps)
+
+
+@pytest.mark.parametrize("dtype,vocab", [("f32", 503), ("f32", 5003), ("f16", 5007), ("bf16", 50023)])
+@pytest.mark.parametrize("depth", [80.0, 86.0, 88.0, 90.0, 96.0])
+def test_cross_entropy_of_rows_whose_last_values_are_far_below_the_others(dtype, vocab, depth):
+    """An odd vocabulary that is padded at its end: the single values are a thread's first."""
+    g = gen(22)
+    x = torch.randn(16, vocab, device="cuda", generator=g)
+    x[:, vocab - 3:] = -depth
+    t = torch.randint(0, vocab, (16,), device="cuda", generator=g)
+    check_rows(x.to(R.TORCH[dtype]), t, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,vocab", [(300, 500), (300, 4096), (300, 5001), (40, 33001)])
+@pytest.mark.parametrize("spread", [15.0, 20.0, 25.0, 30.0, 60.0])
+def test_cross_entropy_of_widely_spread_rows(dtype, rows, vocab, spread):
+    g = gen(23)
+    x = (torch.randn(rows, vocab, device="cuda", generator=g) * spread).to(R.TORCH[dtype])
+    t = torch.randint(0, vocab, (rows,), device="cuda", generator=g)
+    check_rows(x, t, dtype)
+
+
+@pytest.mark.parametrize("scale", [1.0, 2.0 ** -20, 2.0 ** -60])
+def test_gradient_of_a_mean_over_rows_with_one_value_far_above_the_others(scale):
+    """The gradient's factor g / sum is far from f32's limits wherever a thread's reference lies."""
+    g = gen(24)
+    rows, vocab = 8192, 600
+    x = 2.0 * torch.rand(rows, vocab, device="cuda", generator=g)
+    at = torch.arange(rows, device="cuda")
+    x[at, 300 + at % 290] = 80.0 + (at % 7).float()
+    t = torch.randint(0, vocab, (rows,), device="cuda", generator=g)
+    _, _, grad, gbound = R.cross_entropy(x, t, seed=torch.tensor(scale, device="cuda"))
+    X = R.wrap(x)
+    got = ft.grad(F.cross_entropy(X, R.wrap(t)) * scale, X).torch()
+    R.check(got, grad, R.rounded(gbound + FLUSHED * scale / rows, grad, "f32"))
+
+
+def test_cross_entropy_of_rows_far_from_zero():
+    """References beyond 2^24, where whole numbers are no longer all f32 values."""
+    g = gen(25)
+    x = torch.randn(24, 5003, device="cuda", generator=g) * 2.0
+    x[:, :2048] = -90.0
+    x[:, 0] = 0.0
+    far = torch.tensor([0.0, 1e3, -1e4, 1e5, 1e6, -3e6, 8e6, 1.3e7, -2e7, 1e8, 1e12, -1e20], device="cuda").repeat(2)
+    x += far[:, None]
+    t = torch.randint(0, 5003, (24,), device="cuda", generator=g)
+    check_rows(x, t, "f32")
