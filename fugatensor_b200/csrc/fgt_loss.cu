@@ -516,7 +516,8 @@ extern "C" fgt_status fgt_cross_entropy(const fgt_cross_entropy_desc* d, const v
     const LossPlan p = plan_loss(d);
     check_buffer(logits, d->rows * d->vocab, "logits");
     check_buffer(targets, d->rows, "targets");
-    require(loss != nullptr || dlogits != nullptr, "neither loss nor dlogits is asked for");
+    // outputs without elements have no address: with no rows, all but a reduced loss
+    require(loss != nullptr || dlogits != nullptr || d->rows == 0, "neither loss nor dlogits is asked for");
     if (loss) check_buffer(loss, 1, "loss");
     if (dlogits) check_buffer(dlogits, d->rows * d->vocab, "dlogits");
     if (seed) check_buffer(seed, 1, "seed");
@@ -524,6 +525,7 @@ extern "C" fgt_status fgt_cross_entropy(const fgt_cross_entropy_desc* d, const v
                                          std::to_string(p.bytes) + " bytes needed", FGT_ERR_WORKSPACE);
     require(p.bytes == 0 || (workspace && (uintptr_t)workspace % 256 == 0),
             "workspace must be a 256-byte aligned device buffer", FGT_ERR_WORKSPACE);
+    if (d->rows == 0 && (!loss || d->reduction == FGT_LOSS_NONE)) return;  // nothing to write
     check_pending();
     char* ws = (char*)workspace;
     const Launch l{(cudaStream_t)stream, programmatic((cudaStream_t)stream)};

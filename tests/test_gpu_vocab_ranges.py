@@ -101,3 +101,29 @@ def test_cross_entropy_of_rows_far_from_zero():
     x += far[:, None]
     t = torch.randint(0, 5003, (24,), device="cuda", generator=g)
     check_rows(x, t, "f32")
+
+
+# ------------------------------------------------- cross-entropy, no rows --
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("shape", [(0, 40), (2, 0, 40)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_cross_entropy_without_rows(reduction, shape, dtype):
+    X = R.wrap(torch.empty(shape, device="cuda", dtype=R.TORCH[dtype]))
+    T = R.wrap(torch.empty(shape[:-1], device="cuda", dtype=torch.int64))
+
+    def make():
+        loss = F.cross_entropy(X, T, reduction=reduction)
+        seed = R.wrap(torch.ones(shape[:-1], device="cuda")) if reduction == "none" else None
+        return loss, ft.grad(loss, X, seed=seed)
+
+    def check_loss(l):
+        l = l.torch()
+        assert l.shape == (shape[:-1] if reduction == "none" else ()) and not l.any() and l.dtype is torch.float32
+
+    check_loss(make()[0])
+    d = make()[1].torch()
+    assert d.shape == shape and d.dtype is R.TORCH[dtype]
+    l, d = make()
+    ft.evaluate(l, d)
+    check_loss(l)
+    assert d.torch().shape == shape
