@@ -7,6 +7,7 @@ import fugatensor_b200.nn.functional as F
 from tests import _vocab as R
 
 pytestmark = pytest.mark.gpu
+DTYPES = ["f32", "f16", "bf16"]
 
 
 def gen(seed):
@@ -127,3 +128,47 @@ def test_cross_entropy_without_rows(reduction, shape, dtype):
     ft.evaluate(l, d)
     check_loss(l)
     assert d.torch().shape == shape
+
+
+# ------------------------------------------------ logit rules, many biases --
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("index", ["i32", "i64"])
+@pytest.mark.parametrize("rows,vocab,biases", [(3, 40, 513), (2, 5001, 5000), (2, 50021, 40000), (1, 128000, 128000)])
+def test_adjust_logits_with_many_biases(dtype, index, rows, vocab, biases):
+    """Whole numbers, so that sums are exact in any order; with and without a history and a mask."""
+    g = gen(26)
+    x = torch.randint(-30, 31, (rows, vocab), device="cuda", generator=g).to(R.TORCH[dtype])
+    ids = torch.randint(-2, vocab + 2, (rows, biases), device="cuda", generator=g, dtype=R.TORCH[index])
+    ids[:, ::9] = 7  # many for one token
+    bias = torch.randint(-2, 3, (rows, biases), device="cuda", generator=g).float()
+    tokens = torch.randint(0, vocab, (rows, 700), device="cuda", generator=g, dtype=torch.int32)
+    words = torch.randint(-2 ** 31, 2 ** 31, (rows, -(-vocab // 32)), device="cuda", generator=g, dtype=torch.int32)
+    for t, a in ((None, None), (tokens, words)):
+        out = F.adjust_logits(R.wrap(x), None if t is None else R.wrap(t), presence=1.0, frequency=2.0, bias_tokens=R.wrap(ids),
+                              bias=R.wrap(bias), allowed=None if a is None else R.wrap(a)).torch()
+        ref, _ = R.adjust_logits(x, t, presence=1.0, frequency=2.0, bias_tokens=ids, bias=bias, allowed=a)
+        assert torch.equal(out, ref.to(out.dtype))
+
+
+@pytest.mark.parametrize("places", [(0, 1, 2, 3), (0, 31, 32, 33), (5, 700, 1500, 1999), (1, 511, 512, 1024)])
+def test_many_biases_of_one_token_add_in_their_order(places):
+    """2^24 + 1 + 1 - 2^24 in f32, in order, is 0; any other association gives 2."""
+    ids = torch.arange(2000, device="cuda", dtype=torch.int32)[None] % 400 + 100
+    bias = torch.zeros(1, 2000, device="cuda")
+    for p, b in zip(places, (2.0 ** 24, 1.0, 1.0, -2.0 ** 24)):
+        ids[0, p], bias[0, p] = 3, b
+    out = F.adjust_logits(R.wrap(torch.zeros(1, 600, device="cuda")), bias_tokens=R.wrap(ids), bias=R.wrap(bias)).torch()
+    assert not out.any()
+
+
+def test_a_million_biases():
+    """The work grows with the list, not with its square; all for one token, and spread out."""
+    n, vocab = 1 << 20, 128000
+    x = torch.zeros(1, vocab, device="cuda")
+    bias = torch.ones(1, n, device="cuda")
+    one = torch.full((1, n), 77, device="cuda", dtype=torch.int32)
+    out = F.adjust_logits(R.wrap(x), bias_tokens=R.wrap(one), bias=R.wrap(bias)).torch()
+    assert float(out[0, 77]) == n and float(out.sum()) == n
+    each = (torch.arange(n, device="cuda", dtype=torch.int32) % vocab)[None]
+    out = F.adjust_logits(R.wrap(x), bias_tokens=R.wrap(each), bias=R.wrap(bias)).torch()
+    assert torch.equal(out[0], torch.bincount(each[0].long(), minlength=vocab).float())
