@@ -200,6 +200,8 @@ def adjust_logits(logits, tokens=None, lengths=None, *, prompt_lengths=None, rep
     def take(name, x, kinds, shape=None):  # None: the batch's, with a length of its own
         _tensor(x, name, kinds, logits)
         if shape is None:
+            if not x._shape:
+                raise ValueError(f"{name} must have shape {batch} and a length of its own, got ()")
             shape = batch + x._shape[-1:]
         if x._shape != shape:
             raise ValueError(f"{name} must have shape {shape}, got {x._shape}")
