@@ -3,6 +3,8 @@
 // With lse = log(sum_v exp(x_v)) of a row x of logits and its target t:
 //   loss = lse - (1 - e) x_t - (e / V) sum_v x_v + z lse^2
 //   dx_v = g (softmax_v (1 + 2 z lse) - (1 - e) [v = t] - e / V)
+#include <cfloat>
+
 #include "fgt_vocab.cuh"
 
 namespace fgt {
@@ -447,7 +449,7 @@ void check(const fgt_cross_entropy_desc* d) {
   require(is_float(d->dtype), "dtype must be f32, f16 or bf16");
   require(d->reduction >= FGT_LOSS_NONE && d->reduction <= FGT_LOSS_MEAN, "unknown reduction");
   require(d->label_smoothing >= 0.0f && d->label_smoothing <= 1.0f, "label_smoothing must be in [0, 1]");
-  require(d->z_loss >= 0.0f && d->z_loss < 3.4e38f, "z_loss must be finite and not negative");
+  require(d->z_loss >= 0.0f && d->z_loss <= FLT_MAX, "z_loss must be finite and not negative");
   require(d->vocab > 0, "vocab must be positive");
   require(d->vocab <= 1 << 30, "vocab must be at most 2^30");
   size_product(d->rows, d->vocab, "rows x vocab");

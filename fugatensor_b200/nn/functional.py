@@ -13,8 +13,6 @@ has no derivative).
 """
 from __future__ import annotations
 
-import math as _math
-
 from .. import dtypes as _dt
 from .. import operators as _operators
 from .. import ops as _ops
@@ -22,6 +20,7 @@ from ..autograd import stop_gradient
 from ..tensor import Tensor as _Tensor
 
 _FLOAT, _INDEX = ("f32", "f16", "bf16"), ("i32", "i64")
+_F32_OVER, _F32_ZERO = 2.0 ** 128 - 2.0 ** 103, 2.0 ** -150  # f32: infinite from here on; zero down from here
 
 
 def _norm_axes(x, normalized_shape, axis):
@@ -114,10 +113,9 @@ def _tensor(x, what, kinds, like=None):
 def _number(x, what):
     if type(x) not in (int, float):
         raise TypeError(f"{what} must be a number")
-    x = float(x)
-    if not _math.isfinite(x):
-        raise ValueError(f"{what} must be finite")
-    return x
+    if not -_F32_OVER < x < _F32_OVER:
+        raise ValueError(f"{what} must be finite in f32")
+    return float(x)
 
 
 def embedding(table, indices, *, scale=1.0, padding_idx=None):
@@ -227,7 +225,7 @@ def adjust_logits(logits, tokens=None, lengths=None, *, prompt_lengths=None, rep
             numbers.append(1.0)
         else:
             numbers.append(_number(x, name))
-    if numbers[0] <= 0.0:
+    if numbers[0] <= _F32_ZERO:
         raise ValueError("repetition must be positive")
     if (bias is None) != (bias_tokens is None):
         raise ValueError("bias and bias_tokens are given together")
