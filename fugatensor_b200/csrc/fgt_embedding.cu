@@ -808,7 +808,9 @@ extern "C" fgt_status fgt_embedding_grad(const fgt_embedding_desc* d, const void
     check_pending();
     char* ws = (char*)workspace;
     const Launch l{(cudaStream_t)stream, programmatic((cudaStream_t)stream)};
-    const Tokens tk{Index{indices, d->index_dtype == FGT_I64}, (unsigned)d->count, d->vocab, d->padding_index};
+    // a padding row outside the table is none: narrowed to 32 bits it could be another one
+    const int64_t padding = d->padding_index >= 0 && d->padding_index < d->vocab ? d->padding_index : -1;
+    const Tokens tk{Index{indices, d->index_dtype == FGT_I64}, (unsigned)d->count, d->vocab, padding};
     unsigned *keys = (unsigned*)(ws + p.keys), *pos = (unsigned*)(ws + p.pos), *first = (unsigned*)(ws + p.first);
     const Sums s{keys, pos, first, (unsigned long long*)(ws + p.done), (float*)(ws + p.partial), (fgt_u16*)(ws + p.present),
                  (unsigned)d->count, (unsigned)p.tiles, (unsigned)d->vocab};

@@ -372,7 +372,7 @@ typedef struct fgt_embedding_desc {
   int64_t vocab;          /* table rows                                             */
   int64_t dim;            /* row length                                             */
   int64_t count;          /* indices                                                */
-  int64_t padding_index;  /* its row gets no gradient (-1: none)                    */
+  int64_t padding_index;  /* its row gets no gradient (none if outside the table)   */
   float scale;
   int32_t reserved;
 } fgt_embedding_desc;

@@ -4,6 +4,7 @@ import torch
 
 import fugatensor_b200 as ft
 import fugatensor_b200.nn.functional as F
+from fugatensor_b200 import _fgt, _native
 from tests import _vocab as R
 
 pytestmark = pytest.mark.gpu
@@ -172,3 +173,19 @@ def test_a_million_biases():
     each = (torch.arange(n, device="cuda", dtype=torch.int32) % vocab)[None]
     out = F.adjust_logits(R.wrap(x), bias_tokens=R.wrap(each), bias=R.wrap(bias)).torch()
     assert torch.equal(out[0], torch.bincount(each[0].long(), minlength=vocab).float())
+
+
+# -------------------------------------------------- embedding gradient -----
+@pytest.mark.parametrize("index", [torch.int32, torch.int64])
+@pytest.mark.parametrize("padding", [-1, -2 ** 40, 8, 2 ** 32 + 5, 2 ** 33 + 5])
+def test_a_padding_index_outside_the_table_is_none(index, padding):
+    """Straight through the C entry point: the public function refuses it."""
+    ids = torch.tensor([5, 5, 1, 5], device="cuda", dtype=index)
+    dy, out = torch.ones(4, 4, device="cuda"), torch.full((8, 4), -1.0, device="cuda")
+    desc = (3, 1 if index is torch.int32 else 2, 8, 4, 4, 1.0, padding)
+    ws = torch.empty(_native.embedding_grad_workspace(*desc), device="cuda", dtype=torch.uint8)
+    _fgt.check(_native.embedding_grad(*desc, ids.data_ptr(), dy.data_ptr(), out.data_ptr(), ws.data_ptr(), ws.numel(),
+                                      torch.cuda.current_stream().cuda_stream))
+    want = torch.zeros(8, 4, device="cuda")
+    want[5], want[1] = 3.0, 1.0
+    assert torch.equal(out, want)
