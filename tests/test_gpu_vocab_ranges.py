@@ -176,6 +176,26 @@ def test_a_million_biases():
 
 
 # -------------------------------------------------- embedding gradient -----
+TIERS = [1024, 8192, 16384, 32768, 65536, 131072, 1 << 18]  # tokens at which the sort takes another form
+
+
+@pytest.mark.parametrize("n", [m for t in TIERS for m in (t, t + 1)] + [12000, 24000, 200000])
+@pytest.mark.parametrize("vocab", [300, 40000, 300000])  # one, two and three passes
+@pytest.mark.parametrize("dim", [4, 9])
+def test_embedding_grad_in_every_form_of_the_sort(n, vocab, dim):
+    """Whole numbers: the sums are exact. Some tokens are frequent, some have no gradient."""
+    g = gen(27)
+    u = torch.rand(n, device="cuda", generator=g, dtype=torch.float64)
+    ids = ((vocab + 1.0) ** u - 1.0).floor().clamp(0, vocab - 1).to(torch.int64 if n % 2 else torch.int32)
+    ids[::5] = vocab - 1
+    ids[1::97] = -1
+    dy = torch.randint(-3, 4, (n, dim), device="cuda", generator=g).float()
+    table = R.wrap(torch.zeros(vocab, dim, device="cuda"))
+    got = ft.grad(F.embedding(table, R.wrap(ids), padding_idx=2), table, seed=R.wrap(dy)).torch()
+    ref, _ = R.embedding_grad(ids, dy, vocab, 1.0, 2)
+    assert torch.equal(got.double(), ref)
+
+
 @pytest.mark.parametrize("index", [torch.int32, torch.int64])
 @pytest.mark.parametrize("padding", [-1, -2 ** 40, 8, 2 ** 32 + 5, 2 ** 33 + 5])
 def test_a_padding_index_outside_the_table_is_none(index, padding):
