@@ -140,12 +140,12 @@ class Engine:
                 continue
             seen.add(id(t))
             stack.append((t, True))
-            if t._expr is not None and id(t) not in known:
+            if t._expr is not None and not (known and id(t) in known):
                 for a in reversed(t._expr[1]):
                     if id(a) not in seen:
                         stack.append((a, False))
         for t in order:
-            if t._expr is None or id(t) in known:
+            if t._expr is None or known and id(t) in known:
                 v = g.parameter(t.dtype.ir, t.shape)
                 leaves.append(t)
             else:
@@ -198,12 +198,12 @@ class Engine:
                 if r._ops:
                     self._evaluate_operators(roots)
                     return tensors[0] if len(tensors) == 1 else tensors
-            import torch
-            from . import _fgt
-            desc, leaves, roots = self._trace(roots, {})
             if not roots:
                 return tensors[0] if len(tensors) == 1 else tensors
+            desc, leaves, roots = self._trace(roots, {})
+            import torch
             if not torch.cuda.is_available():
+                from . import _fgt
                 raise _fgt.CUDAError(4, "no CUDA device: fugatensor_b200 has no CPU execution path")
             device = torch.device(self.device)
             with torch.cuda.device(device):
@@ -218,7 +218,7 @@ class Engine:
         from . import _fgt
         spec = self._spec(desc)
         prog = self._program(desc.key(), spec)
-        inputs = [known[id(t)] if id(t) in known else t._data for t in leaves]
+        inputs = [known[id(t)] if known and id(t) in known else t._data for t in leaves]
         outs = _fgt.run(spec, *[x if x.device == device else x.to(device) for x in inputs], program=prog)
         plan = dict(spec.execution_plan)
         lowering = plan.pop("cuda_lowering")

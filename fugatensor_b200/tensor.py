@@ -389,7 +389,7 @@ def _index_op(g, op, vals, attrs):
 
 def _prim(op, args, attrs=()):
     """A pending tensor for primitive `op` over `args`."""
-    engine = None
+    engine, operators = None, False
     for a in args:
         if not isinstance(a, Tensor):
             raise TypeError(f"{op} operands must be Tensors")
@@ -397,9 +397,12 @@ def _prim(op, args, attrs=()):
             engine = a._engine
         elif a._engine is not engine:
             raise ValueError("tensors belong to different engines")
+        if a._ops:
+            operators = True
     dtype, shape = _infer(op, args, attrs)
     t = Tensor(engine, _dt.BY_IR[dtype], shape, expr=(op, tuple(args), tuple(attrs)))
-    t._ops = any(a._ops for a in args)
+    if operators:
+        t._ops = True
     return t
 
 
