@@ -157,7 +157,9 @@ enum Group { kWarp, kCta, kCluster };
 constexpr int kBatch = 4, kStages = 3;  // 192 bytes per thread: 1024 threads keep 128 KB in flight per SM
 constexpr int kWarpGroups = 4;          // warps of a CTA that has a row per warp
 
-// The sum of exponentials is 2^c s with a whole c, else e^c s (c = -inf where s = 0); the sum of x.
+// The sum of exponentials is 2^c s with a whole c, else e^c s (c = -inf where s =
+// 0); the sum of (e / V) x, each by itself: that of x overflows where a few columns
+// are masked with the type's lowest value.
 struct Stat {
   float c, s, all;
 };
@@ -330,14 +332,14 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
       stat.c = reference(now.x_single);
       sum[0] = Exponent<true>(stat.c)(make_float2(now.x_single, kNegInf));
     }
-    if (now.single >= 0) all.x = now.x_single;
+    if (kAll && now.single >= 0) all.x = __fmul_rn(smoothed, now.x_single);
     Exponent<true> exp2(stat.c);
     each(end - first, [&](int b, const uint4& u) {
       float v[N];
       Vec<T>::unpack(u, v);
       if (kAll)
 #pragma unroll
-        for (int e = 0; e < N; e += 2) all = __fadd2_rn(all, make_float2(v[e], v[e + 1]));
+        for (int e = 0; e < N; e += 2) all = __ffma2_rn(both(smoothed), make_float2(v[e], v[e + 1]), all);
       if (stat.c == kNegInf) {
         float m = v[0];
 #pragma unroll
@@ -408,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
     if (tells || r.z != 0.0f) lse = whole ? (stat.c + log2f(stat.s)) * kLn2 : stat.c + logf(stat.s);
     if (tells) {
       float l = lse - (1.0f - r.smoothing) * now.x_t;
-      if (kAll) l -= smoothed * stat.all;
+      if (kAll) l -= stat.all;
       if (r.z != 0.0f) l += r.z * lse * lse;
       losses[row] = l;
     }

@@ -105,6 +105,17 @@ def test_cross_entropy_of_rows_far_from_zero():
     check_rows(x, t, "f32")
 
 
+@pytest.mark.parametrize("dtype,vocab", [("f32", 515), ("f32", 5003), ("bf16", 600), ("bf16", 40001)])
+def test_smoothed_loss_of_columns_at_the_lowest_value(dtype, vocab):
+    """(e / vocab) * sum(x) is far inside f32 although sum(x) is not."""
+    g = gen(28)
+    x = torch.randn(6, vocab, device="cuda", generator=g).to(R.TORCH[dtype])
+    x[:, vocab // 3:vocab // 2] = torch.finfo(x.dtype).min
+    x[1, vocab - 1] = torch.finfo(x.dtype).min
+    t = torch.randint(0, vocab // 3, (6,), device="cuda", generator=g)
+    check_rows(x, t, dtype, eps=0.1)
+
+
 # ------------------------------------------------- cross-entropy, no rows --
 @pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
 @pytest.mark.parametrize("shape", [(0, 40), (2, 0, 40)])
