@@ -1,16 +1,17 @@
 // fgt_embedding.cu — embedding lookup with scaling, and its gradient.
 //
 //   out[i, :]    = s * table[t_i, :]               (0 where t_i is outside [0, V))
-//   dtable[v, :] = s * sum over {i : t_i = v} of dy[i, :], in the order of i
+//   dtable[v, :] = s * sum over {i : t_i = v} of dy[i, :]
 //
 // Both are bound by memory: the lookup reads its rows and writes them, the
 // gradient reads dy once and writes the whole table once. What is hard in the
 // gradient is the skew of text: a few tokens make up a large share of a batch
 // while most rows of the table get none, and adding rows with atomics would
 // make the result depend on their order. So the (token, position) pairs are
-// sorted (stable, hence in the order of i), long runs of one token are cut into
-// pieces that different warps add in f32, and the last warp to finish adds the
-// pieces in their order; rows without a token are zeroed while the sort runs.
+// sorted (stable) and a token's rows are added in the order of i; runs of more
+// than 64 are cut into pieces that different warps add in f32, and the last warp
+// to finish adds the pieces' sums in their order, whichever warp that is. Rows
+// without a token are zeroed while the sort runs.
 #include <type_traits>
 
 #include "fgt_vocab.cuh"

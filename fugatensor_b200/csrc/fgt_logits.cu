@@ -10,7 +10,7 @@
 // after the others, one thread each; longer lists of biases (kMany) are summed in
 // shared memory, in their order.
 // On B200 64 rows of 128000 bf16 with up to 4096 tokens, 32 biases and a mask
-// take 17 us (a copy of them 9: the rest is a chain of loads and barriers), 384
+// take 18 us (a copy of them 9: the rest is a chain of loads and barriers), 384
 // rows of 50021 f32 with up to 32768 tokens and 300 biases 55 us (a copy 24: the
 // rest is instructions, half of them for the history, which every slice reads).
 // Registers are what it is short of: three CTAs per SM leave 40 per thread, and

@@ -147,12 +147,17 @@ __global__ void __launch_bounds__(kCountThreads)
 // to 2 (N - 1) single values, one for each of the group's first threads.
 // Bound by memory for f32 and long rows, by instructions (two exponentials a
 // value, and about 300 instructions per warp and row) for 16-bit and short
-// ones. On B200: 4096 x 32000 f32, loss alone, 82 us (0.98 of a copy's rate);
-// 2048 x 128000 f32 with the gradient 370 us (0.87); 8192 x 128000 bf16 677 us
-// (0.95), 740 to 790 where the power cap has lowered the clock; 8192 x 32000
-// bf16 188 us (0.85); 2048 x 50021 f16 93 us (0.67). Rows held in registers,
-// shared by a cluster, took 1250 us for the bf16 case (each phase waits for the
-// one before); a ring of whole row slices per cluster 1350 to 3400 us.
+// ones. Calls in a row on B200: 4096 x 32000 f32, loss alone, 87 us (0.92 of a
+// copy's rate); 2048 x 128000 f32 with the gradient 387 us (0.83); 8192 x 128000
+// bf16 777 us (0.82) under the power cap's clock, 683 before it sets in; 8192 x
+// 32000 bf16 196 to 204 us (0.8); 2048 x 50021 f16 100 us (0.63). Rows held in
+// registers, shared by a cluster, took 1250 us for the bf16 case (each phase
+// waits for the one before); a ring of whole row slices per cluster 1350 to 3400.
+// The second attempt reads a row twice more, one vector per thread at a time and
+// outside the ring. Where it meets every row (normal logits with a deviation of
+// 30, or a sixteenth of the columns at -1e4) these take 177, 560, 1085, 300 and
+// 150 us; a few columns at -1e4 at the end of an odd vocabulary, the single
+// values, 145 us in place of 113 for 2048 x 50021 f16.
 enum Group { kWarp, kCta, kCluster };
 constexpr int kBatch = 4, kStages = 3;  // 192 bytes per thread: 1024 threads keep 128 KB in flight per SM
 constexpr int kWarpGroups = 4;          // warps of a CTA that has a row per warp

@@ -123,8 +123,9 @@ def embedding(table, indices, *, scale=1.0, padding_idx=None):
 
     Indices outside [0, vocab) read a row of zeros and take no part in the
     gradient (as in ``gather``). The gradient of ``table`` adds the cotangent's
-    rows in the order of their indices, in f32, and rounds once; the row
-    ``padding_idx`` gets none.
+    rows in f32 and rounds once: in the order of their indices, for an index that
+    occurs more than 64 times in fixed pieces of 64 whose sums are then added in
+    order. The row ``padding_idx`` gets none.
     """
     _tensor(table, "embedding table", _FLOAT)
     _tensor(indices, "embedding indices", _INDEX, table)
@@ -148,8 +149,8 @@ def cross_entropy(logits, targets, *, ignore_index=-100, label_smoothing=0.0, z_
     target is ``ignore_index`` or outside [0, vocab) have loss 0 and gradient 0
     and do not count in the mean (0 when no row counts). A counted row whose
     logits are all -inf has no distribution: its loss and gradient are NaN.
-    Evaluated together with its ``ft.grad``, loss and gradient are one pass
-    that reads the logits once.
+    Evaluated together with its ``ft.grad``, loss and gradient are one launch
+    that reads the logits from memory once.
     """
     _tensor(logits, "cross_entropy logits", _FLOAT)
     _tensor(targets, "cross_entropy targets", _INDEX, logits)

@@ -7,7 +7,7 @@ its gradient, the rules that edit logits. ``Engine.evaluate`` cuts the graph
 at them: whatever an operator reads is evaluated first (as partitions and
 operators), and partitions take operator results as inputs. A loss and its
 gradient that are evaluated together run as one launch that reads the logits
-once.
+from memory once.
 
 The public functions are in ``nn.functional``; this module types the nodes,
 gives their VJPs and launches them. Like partitions they run on the current

@@ -410,8 +410,10 @@ typedef struct fgt_cross_entropy_desc {
  * rows' number (MEAN; 0 when no row counts). seed is f32, the loss's
  * cotangent: [rows] for NONE, one value otherwise, or NULL for 1; g_i is
  * grad_scale * seed, over the number of counted rows for MEAN. loss or
- * dlogits may be NULL (not computed; with no rows, both may); with both, the
- * logits are read once. */
+ * dlogits may be NULL (not computed; with no rows, both may). With both, the
+ * logits are read from memory once; the gradient's reading finds them in L2. A
+ * row whose largest logits lie about 88 and more above those that its threads
+ * read first is read twice more. */
 fgt_status fgt_cross_entropy_workspace(const fgt_cross_entropy_desc* desc, size_t* bytes);
 fgt_status fgt_cross_entropy(const fgt_cross_entropy_desc* desc, const void* logits, const void* targets,
                              const float* seed, float* loss, void* dlogits, void* workspace, size_t workspace_bytes,
